@@ -537,6 +537,119 @@ rl_status rl_gqa_pv_matmul_f16(rl_context* ctx, const rl_buffer* probs, const rl
                                uint64_t q_len, uint64_t kv_len, uint64_t head_dim,
                                uint64_t kv_capacity, const rl_buffer* out);
 
+/* =========================================== serving a batch of requests */
+/* No counterpart in the reference, whose cache holds one sequence in max_seq
+ * rows (src/model/kv_cache.rs) and whose attention takes one length a call.
+ * Requests of different lengths share a cache of pages: [pages, kv_heads,
+ * page_size, head_dim], K and V each, page_size a power of two and pages *
+ * page_size below 2^32.  Request i's position p lives in page
+ * block_table[i, p / page_size], row p % page_size; its slot is page *
+ * page_size + row.  Lengths, tables, offsets, slots and positions are device
+ * buffers of 32-bit unsigned values, read when the kernels run: a recorded
+ * step follows what its replay finds in them.  Row ranges, pages and slots
+ * that lie outside their buffers are never followed (each entry says what
+ * comes out).  The batch's tokens are rows: request i owns rows offsets[i] ..
+ * offsets[i + 1] of every [tokens, heads, head_dim] tensor. */
+#define RL_NO_PAGE 0xffffffffu
+#define RL_NO_SLOT 0xffffffffu
+
+/* A step's plan from the requests' lengths.  Request i has cached[i] tokens in
+ * the cache, their pages in the first ceil(cached[i] / page_size) entries of
+ * its table row, and fresh[i] new ones (0 allowed).
+ *   offsets[0 .. sequences]: sums of fresh; context[i] = cached[i] + fresh[i]
+ *   block_table: entries ceil(cached / page_size) .. ceil(context / page_size)
+ *     of each row (as far as max_blocks) take the next pages of free_pages, in
+ *     request order; RL_NO_PAGE once those are used up.  Others are kept.
+ *   positions[t], slots[t]: of each new token, in request order; 0 and
+ *     RL_NO_SLOT for a token whose page is missing, at or past `pages` or past
+ *     the table row, and for rows behind the last request's
+ *   taken[0]: pages needed; more than free_pages holds = some tokens have none
+ * `tokens` (the length of slots and positions) is at least the sum of fresh;
+ * tokens past it, and pages that start past it, are not planned.  Sums stop at
+ * 2^32 - 1. */
+rl_status rl_paged_plan(rl_context* ctx, const rl_buffer* cached, const rl_buffer* fresh,
+                        uint64_t sequences, const rl_buffer* free_pages,
+                        const rl_buffer* block_table, uint64_t max_blocks, uint64_t pages,
+                        uint64_t page_size, const rl_buffer* offsets, const rl_buffer* context,
+                        uint64_t tokens, const rl_buffer* slots, const rl_buffer* positions,
+                        const rl_buffer* taken);
+
+/* rl_qkv_rope_kv_append_* for a paged cache: q/k/v are [tokens, heads, D] views
+ * (dims and strides of rank 3, unit innermost strides: the parts of a
+ * projection's rows); Q, rotated at positions[t], goes to the contiguous
+ * [tokens, QH, D] q_out, K, rotated, and V to row slots[t] of their pages.  A
+ * token whose slot is outside the pool (RL_NO_SLOT) or whose position is at or
+ * past table_rows is skipped: nothing of it is written.  No two tokens may
+ * share a slot.  Same rotation, bit for bit, as rl_rope_*. */
+rl_status rl_qkv_rope_paged_append_f32(
+    rl_context* ctx, const rl_buffer* q_src, const uint64_t* q_dims, const uint64_t* q_strides,
+    const rl_buffer* k_src, const uint64_t* k_dims, const uint64_t* k_strides,
+    const rl_buffer* v_src, const uint64_t* v_dims, const uint64_t* v_strides,
+    const rl_buffer* cos_table, const rl_buffer* sin_table, uint64_t table_rows,
+    const rl_buffer* positions, const rl_buffer* slots, const rl_buffer* q_out,
+    const rl_buffer* k_pages, const rl_buffer* v_pages, uint64_t pages, uint64_t page_size);
+rl_status rl_qkv_rope_paged_append_f16(
+    rl_context* ctx, const rl_buffer* q_src, const uint64_t* q_dims, const uint64_t* q_strides,
+    const rl_buffer* k_src, const uint64_t* k_dims, const uint64_t* k_strides,
+    const rl_buffer* v_src, const uint64_t* v_dims, const uint64_t* v_strides,
+    const rl_buffer* cos_table, const rl_buffer* sin_table, uint64_t table_rows,
+    const rl_buffer* positions, const rl_buffer* slots, const rl_buffer* q_out,
+    const rl_buffer* k_pages, const rl_buffer* v_pages, uint64_t pages, uint64_t page_size);
+
+/* Memory for rl_paged_attention_* calls of up to these sizes (release it with
+ * rl_buffer_release).  It serves one call at a time: calls that may overlap
+ * (contexts on other streams) need one each; calls in order on one context,
+ * and graphs replayed on it, can share one.  Not while recording. */
+rl_status rl_paged_attention_workspace(rl_context* ctx, uint64_t sequences, uint64_t tokens,
+                                       uint64_t q_heads, uint64_t kv_heads, uint64_t head_dim,
+                                       rl_buffer* out);
+/* rl_attention_* of every request's new tokens over its pages, single tokens
+ * and chunks in one call: row offsets[i] + j is request i's position
+ * context[i] - n + j (n its rows) and sees the keys at positions up to its
+ * own.  q, out: contiguous [tokens, q_heads, head_dim].  No request has more
+ * than max_queries rows or max_context positions (at most max_blocks *
+ * page_size).  Rows of no request (and past a request's first max_queries)
+ * are not written; a row that sees no key (a position below 0) is zeros; a
+ * row that sees a key of a page at or past `pages`, and every row of a
+ * request whose context passes max_context, is NaN.  Types, roundings and
+ * head sizes as rl_attention_*.  May be recorded into a graph, the workspace
+ * made before. */
+rl_status rl_paged_attention_f32(rl_context* ctx, const rl_buffer* q, const rl_buffer* k_pages,
+                                 const rl_buffer* v_pages, const rl_buffer* block_table,
+                                 const rl_buffer* offsets, const rl_buffer* context,
+                                 uint64_t sequences, uint64_t tokens, uint64_t q_heads,
+                                 uint64_t kv_heads, uint64_t head_dim, uint64_t pages,
+                                 uint64_t page_size, uint64_t max_blocks, uint64_t max_queries,
+                                 uint64_t max_context, float scale, const rl_buffer* workspace,
+                                 const rl_buffer* out);
+rl_status rl_paged_attention_f16(rl_context* ctx, const rl_buffer* q, const rl_buffer* k_pages,
+                                 const rl_buffer* v_pages, const rl_buffer* block_table,
+                                 const rl_buffer* offsets, const rl_buffer* context,
+                                 uint64_t sequences, uint64_t tokens, uint64_t q_heads,
+                                 uint64_t kv_heads, uint64_t head_dim, uint64_t pages,
+                                 uint64_t page_size, uint64_t max_blocks, uint64_t max_queries,
+                                 uint64_t max_context, float scale, const rl_buffer* workspace,
+                                 const rl_buffer* out);
+/* rl_attention_* over whole prompts packed one after another: row offsets[i] +
+ * j sees rows offsets[i] .. offsets[i] + j.  q/k/v: [tokens, heads, D] views as
+ * rl_qkv_rope_paged_append_* takes them; out: contiguous [tokens, QH, D].  No
+ * prompt has more than max_queries rows (rows past them, and rows of no
+ * prompt, are not written). */
+rl_status rl_packed_attention_f32(rl_context* ctx, const rl_buffer* q, const uint64_t* q_dims,
+                                  const uint64_t* q_strides, const rl_buffer* k,
+                                  const uint64_t* k_dims, const uint64_t* k_strides,
+                                  const rl_buffer* v, const uint64_t* v_dims,
+                                  const uint64_t* v_strides, const rl_buffer* offsets,
+                                  uint64_t sequences, uint64_t max_queries, float scale,
+                                  const rl_buffer* out);
+rl_status rl_packed_attention_f16(rl_context* ctx, const rl_buffer* q, const uint64_t* q_dims,
+                                  const uint64_t* q_strides, const rl_buffer* k,
+                                  const uint64_t* k_dims, const uint64_t* k_strides,
+                                  const rl_buffer* v, const uint64_t* v_dims,
+                                  const uint64_t* v_strides, const rl_buffer* offsets,
+                                  uint64_t sequences, uint64_t max_queries, float scale,
+                                  const rl_buffer* out);
+
 #ifdef __cplusplus
 }
 #endif

@@ -26,6 +26,10 @@ pub const RL_ERR_MODEL_FORMAT: rl_status = 8; // TinyError::ModelFormat
 pub const RL_ERR_DEVICE: rl_status = 9; // TinyError::Metal
 pub const RL_ERR_INVALID_TOKEN_ID: rl_status = 10; // TinyError::InvalidTokenId { .. }
 
+/// Marks a table entry without a page and a token without a slot.
+pub const RL_NO_PAGE: u32 = 0xffff_ffff;
+pub const RL_NO_SLOT: u32 = 0xffff_ffff;
+
 #[repr(C)]
 pub struct rl_context {
     _private: [u8; 0],
@@ -665,6 +669,155 @@ extern "C" {
         kv_len: u64,
         head_dim: u64,
         kv_capacity: u64,
+        out: *const rl_buffer,
+    ) -> rl_status;
+    // a batch of requests over a paged cache (no counterpart in the reference)
+    pub fn rl_paged_plan(
+        ctx: *mut rl_context,
+        cached: *const rl_buffer,
+        fresh: *const rl_buffer,
+        sequences: u64,
+        free_pages: *const rl_buffer,
+        block_table: *const rl_buffer,
+        max_blocks: u64,
+        pages: u64,
+        page_size: u64,
+        offsets: *const rl_buffer,
+        context: *const rl_buffer,
+        tokens: u64,
+        slots: *const rl_buffer,
+        positions: *const rl_buffer,
+        taken: *const rl_buffer,
+    ) -> rl_status;
+    pub fn rl_qkv_rope_paged_append_f32(
+        ctx: *mut rl_context,
+        q_src: *const rl_buffer,
+        q_dims: *const u64,
+        q_strides: *const u64,
+        k_src: *const rl_buffer,
+        k_dims: *const u64,
+        k_strides: *const u64,
+        v_src: *const rl_buffer,
+        v_dims: *const u64,
+        v_strides: *const u64,
+        cos_table: *const rl_buffer,
+        sin_table: *const rl_buffer,
+        table_rows: u64,
+        positions: *const rl_buffer,
+        slots: *const rl_buffer,
+        q_out: *const rl_buffer,
+        k_pages: *const rl_buffer,
+        v_pages: *const rl_buffer,
+        pages: u64,
+        page_size: u64,
+    ) -> rl_status;
+    pub fn rl_qkv_rope_paged_append_f16(
+        ctx: *mut rl_context,
+        q_src: *const rl_buffer,
+        q_dims: *const u64,
+        q_strides: *const u64,
+        k_src: *const rl_buffer,
+        k_dims: *const u64,
+        k_strides: *const u64,
+        v_src: *const rl_buffer,
+        v_dims: *const u64,
+        v_strides: *const u64,
+        cos_table: *const rl_buffer,
+        sin_table: *const rl_buffer,
+        table_rows: u64,
+        positions: *const rl_buffer,
+        slots: *const rl_buffer,
+        q_out: *const rl_buffer,
+        k_pages: *const rl_buffer,
+        v_pages: *const rl_buffer,
+        pages: u64,
+        page_size: u64,
+    ) -> rl_status;
+    pub fn rl_paged_attention_workspace(
+        ctx: *mut rl_context,
+        sequences: u64,
+        tokens: u64,
+        q_heads: u64,
+        kv_heads: u64,
+        head_dim: u64,
+        out: *mut rl_buffer,
+    ) -> rl_status;
+    pub fn rl_paged_attention_f32(
+        ctx: *mut rl_context,
+        q: *const rl_buffer,
+        k_pages: *const rl_buffer,
+        v_pages: *const rl_buffer,
+        block_table: *const rl_buffer,
+        offsets: *const rl_buffer,
+        context: *const rl_buffer,
+        sequences: u64,
+        tokens: u64,
+        q_heads: u64,
+        kv_heads: u64,
+        head_dim: u64,
+        pages: u64,
+        page_size: u64,
+        max_blocks: u64,
+        max_queries: u64,
+        max_context: u64,
+        scale: f32,
+        workspace: *const rl_buffer,
+        out: *const rl_buffer,
+    ) -> rl_status;
+    pub fn rl_paged_attention_f16(
+        ctx: *mut rl_context,
+        q: *const rl_buffer,
+        k_pages: *const rl_buffer,
+        v_pages: *const rl_buffer,
+        block_table: *const rl_buffer,
+        offsets: *const rl_buffer,
+        context: *const rl_buffer,
+        sequences: u64,
+        tokens: u64,
+        q_heads: u64,
+        kv_heads: u64,
+        head_dim: u64,
+        pages: u64,
+        page_size: u64,
+        max_blocks: u64,
+        max_queries: u64,
+        max_context: u64,
+        scale: f32,
+        workspace: *const rl_buffer,
+        out: *const rl_buffer,
+    ) -> rl_status;
+    pub fn rl_packed_attention_f32(
+        ctx: *mut rl_context,
+        q: *const rl_buffer,
+        q_dims: *const u64,
+        q_strides: *const u64,
+        k: *const rl_buffer,
+        k_dims: *const u64,
+        k_strides: *const u64,
+        v: *const rl_buffer,
+        v_dims: *const u64,
+        v_strides: *const u64,
+        offsets: *const rl_buffer,
+        sequences: u64,
+        max_queries: u64,
+        scale: f32,
+        out: *const rl_buffer,
+    ) -> rl_status;
+    pub fn rl_packed_attention_f16(
+        ctx: *mut rl_context,
+        q: *const rl_buffer,
+        q_dims: *const u64,
+        q_strides: *const u64,
+        k: *const rl_buffer,
+        k_dims: *const u64,
+        k_strides: *const u64,
+        v: *const rl_buffer,
+        v_dims: *const u64,
+        v_strides: *const u64,
+        offsets: *const rl_buffer,
+        sequences: u64,
+        max_queries: u64,
+        scale: f32,
         out: *const rl_buffer,
     ) -> rl_status;
 }

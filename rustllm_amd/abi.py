@@ -173,7 +173,23 @@ SIGNATURES: dict[str, tuple[list, object]] = {
     "rl_gqa_qk_matmul_f16": ([_P, _BUF, _BUF] + [_U64] * 7 + [_BUF], _I32),
     "rl_gqa_pv_matmul_f32": ([_P, _BUF, _BUF] + [_U64] * 7 + [_BUF], _I32),
     "rl_gqa_pv_matmul_f16": ([_P, _BUF, _BUF] + [_U64] * 7 + [_BUF], _I32),
+    "rl_paged_plan": ([_P, _BUF, _BUF, _U64, _BUF, _BUF, _U64, _U64, _U64, _BUF, _BUF, _U64, _BUF,
+                       _BUF, _BUF], _I32),
+    "rl_qkv_rope_paged_append_f32": ([_P] + [_BUF, _U64P, _U64P] * 3 + [_BUF, _BUF, _U64]
+                                     + [_BUF] * 5 + [_U64] * 2, _I32),
+    "rl_qkv_rope_paged_append_f16": ([_P] + [_BUF, _U64P, _U64P] * 3 + [_BUF, _BUF, _U64]
+                                     + [_BUF] * 5 + [_U64] * 2, _I32),
+    "rl_paged_attention_workspace": ([_P] + [_U64] * 5 + [_BUF], _I32),
+    "rl_paged_attention_f32": ([_P] + [_BUF] * 6 + [_U64] * 10 + [_F, _BUF, _BUF], _I32),
+    "rl_paged_attention_f16": ([_P] + [_BUF] * 6 + [_U64] * 10 + [_F, _BUF, _BUF], _I32),
+    "rl_packed_attention_f32": ([_P] + [_BUF, _U64P, _U64P] * 3 + [_BUF, _U64, _U64, _F, _BUF],
+                                _I32),
+    "rl_packed_attention_f16": ([_P] + [_BUF, _U64P, _U64P] * 3 + [_BUF, _U64, _U64, _F, _BUF],
+                                _I32),
 }
+
+# A table entry without a page, a token without a slot.
+NO_PAGE = NO_SLOT = 0xFFFFFFFF
 
 _lib: ctypes.CDLL | None = None
 
@@ -251,6 +267,10 @@ def _function(lib, op: str, f16: bool):
     return fn
 
 
+def _power_of_two(n: int) -> int:
+    return 1 << max(n - 1, 0).bit_length()
+
+
 class DeviceBuffer:
     """One pooled rl_buffer with the dtype/shape it was created for."""
 
@@ -307,6 +327,7 @@ class Context:
         handle = ctypes.c_void_p()
         check(self.lib.rl_context_create(device, ctypes.byref(handle)))
         self.handle = handle
+        self._workspaces: dict = {}  # paged_attention's, by sizes
 
     def close(self) -> None:
         if self.handle:
@@ -601,4 +622,75 @@ class Context:
         out = out or self.empty((ids.size, hidden), weight.dtype)
         self._call("embedding", weight, weight, vocab, hidden,
                    ids.ctypes.data_as(ctypes.POINTER(ctypes.c_uint32)), ids.size, out)
+        return out
+
+    # ------------------------------------------ a batch over a paged cache
+    def paged_plan(self, cached, fresh, free_pages, table, page_size: int, pages: int,
+                   offsets=None, context=None, slots=None, positions=None, taken=None,
+                   tokens=None):
+        """One step's offsets, context lengths, slots, positions and count of
+        pages needed from the requests' lengths; new pages go into `table`
+        [requests, max_blocks] (in place).  `tokens` (at least the sum of
+        `fresh`) or `slots` sets the rows of the batch."""
+        requests, blocks = table.shape
+        offsets = offsets or self.empty((requests + 1,), np.uint32)
+        context = context or self.empty((requests,), np.uint32)
+        if slots is None:
+            slots = self.empty((tokens if positions is None else positions.len,), np.uint32)
+        positions = positions or self.empty((slots.len,), np.uint32)
+        taken = taken or self.empty((1,), np.uint32)
+        check(self.lib.rl_paged_plan(self.handle, cached, fresh, requests, free_pages, table,
+                                     blocks, pages, page_size, offsets, context, slots.len, slots,
+                                     positions, taken))
+        return offsets, context, slots, positions, taken
+
+    def qkv_rope_paged_append(self, q, k, v, cos, sin, positions, slots, k_pages, v_pages,
+                              q_out=None):
+        """q/k/v: (buffer, dims, strides) of [tokens, heads, D] views.  Returns
+        the rotated contiguous Q; K (rotated) and V land in their slots of the
+        [pages, KVH, page_size, D] pools."""
+        (qb, qd, qs), (kb, kd, ks), (vb, vd, vs) = q, k, v
+        q_out = q_out or self.empty(qd, qb.dtype)
+        self._call("qkv_rope_paged_append", qb, qb, _u64_array(qd), _u64_array(qs), kb,
+                   _u64_array(kd), _u64_array(ks), vb, _u64_array(vd), _u64_array(vs), cos, sin,
+                   cos.shape[0], positions, slots, q_out, k_pages, v_pages, k_pages.shape[0],
+                   k_pages.shape[2])
+        return q_out
+
+    def paged_workspace(self, sequences: int, tokens: int, q_heads: int, kv_heads: int,
+                        head_dim: int) -> DeviceBuffer:
+        """Memory for paged_attention() calls of up to these sizes, one at a time."""
+        raw = RlBuffer()
+        check(self.lib.rl_paged_attention_workspace(self.handle, sequences, tokens, q_heads,
+                                                    kv_heads, head_dim, ctypes.byref(raw)))
+        return DeviceBuffer(self, raw, np.uint8, (raw.len,))
+
+    def paged_attention(self, q, k_pages, v_pages, table, offsets, context, scale: float,
+                        max_queries: int, max_context: int, out=None, workspace=None):
+        """Attention of each request's rows of q [tokens, QH, D] over its pages
+        of the [pages, KVH, page_size, D] pools.  Without a `workspace` the
+        context makes and keeps its own, one for each power of two of requests
+        and rows (so a step to be recorded runs once before)."""
+        tokens, qh, hd = q.shape
+        pages, kvh, page_size, _ = k_pages.shape
+        requests, blocks = table.shape
+        out = out or self.empty(q.shape, q.dtype)
+        if workspace is None:
+            sizes = (_power_of_two(requests), _power_of_two(tokens), qh, kvh, hd)
+            workspace = self._workspaces.get(sizes)
+            if workspace is None:
+                workspace = self._workspaces[sizes] = self.paged_workspace(*sizes)
+        self._call("paged_attention", q, q, k_pages, v_pages, table, offsets, context, requests,
+                   tokens, qh, kvh, hd, pages, page_size, blocks, max_queries, max_context, scale,
+                   workspace, out)
+        return out
+
+    def packed_attention(self, q, k, v, offsets, scale: float, max_queries: int, out=None):
+        """Causal attention within each packed prompt; q/k/v: (buffer, dims,
+        strides) of [tokens, heads, D] views."""
+        (qb, qd, qs), (kb, kd, ks), (vb, vd, vs) = q, k, v
+        out = out or self.empty(qd, qb.dtype)
+        self._call("packed_attention", qb, qb, _u64_array(qd), _u64_array(qs), kb,
+                   _u64_array(kd), _u64_array(ks), vb, _u64_array(vd), _u64_array(vs), offsets,
+                   offsets.len - 1, max_queries, scale, out)
         return out

@@ -29,7 +29,7 @@ PROBE = os.path.join(PKG, "hbm_probe")
 ARCH = "gfx950"
 HIP_SOURCES = ["runtime.hip", "elementwise.hip", "movement.hip", "rmsnorm.hip", "softmax.hip",
                "rope.hip", "kvcache.hip", "embedding.hip", "attention.hip",
-               "gqa.hip"]
+               "gqa.hip", "paged.hip", "ragged_attention.hip"]
 
 
 def hipcc() -> str:

@@ -120,6 +120,10 @@ struct rl_context {
     uint32_t* tickets = nullptr;
     uint64_t ticket_count = 0;
 
+    // Workspaces that rl_paged_attention_workspace made (address -> bytes) and
+    // that have not been released.
+    std::unordered_map<void*, uint64_t> workspaces;
+
     // Streaming ops recorded into a graph but not yet launched (at most
     // kMaxFused, no two touching the same bytes unless both only read them).
     rl::FusedOp fused[rl::kMaxFused];

@@ -388,6 +388,7 @@ rl_status rl_buffer_copy(rl_context* ctx, const rl_buffer* src, const rl_buffer*
 
 void rl_buffer_release(rl_context* ctx, rl_buffer* buffer) {
     if (ctx == nullptr || buffer == nullptr || buffer->data == nullptr) return;
+    ctx->workspaces.erase(buffer->data);
     ctx->pool.release(buffer->data);
     *buffer = rl_buffer{nullptr, 0, 0};
 }
