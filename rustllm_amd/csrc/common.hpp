@@ -120,9 +120,14 @@ struct rl_context {
     uint32_t* tickets = nullptr;
     uint64_t ticket_count = 0;
 
-    // Workspaces that rl_paged_attention_workspace made (address -> bytes) and
-    // that have not been released.
-    std::unordered_map<void*, uint64_t> workspaces;
+    // Workspaces that rl_paged_attention_workspace made and that have not been
+    // released, by address: first the hand-over counters, zero between calls,
+    // then room for partials.
+    struct Workspace {
+        uint64_t ticket_bytes;
+        uint64_t partial_bytes;
+    };
+    std::unordered_map<void*, Workspace> workspaces;
 
     // Streaming ops recorded into a graph but not yet launched (at most
     // kMaxFused, no two touching the same bytes unless both only read them).

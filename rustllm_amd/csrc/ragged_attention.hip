@@ -16,10 +16,12 @@
 // a query that sees no key (position below 0) as zeros.  Rows of no request
 // are not written.
 #include "common.hpp"
+#include "mfma_layout.hpp"
 #include "ragged.hpp"
 
 #include <algorithm>
 #include <cmath>
+#include <type_traits>
 
 namespace rl {
 namespace {
@@ -46,6 +48,17 @@ struct RaggedParams {
     uint64_t v_token, v_head;
     float scale;
     float scale_log2;  // scale * log2(e)
+    // Requests of at most this many rows a KV head (tokens times group) belong
+    // to the split kernel: it takes those, the others skip them.
+    uint32_t small_rows;
+    // split kernel
+    uint32_t splits;       // workgroups a KV head has for its requests' key ranges
+    uint32_t share;        // key units a KV head's workgroups are sized for
+    uint32_t page_bytes;   // of one page, all KV heads
+    uint32_t head_bytes;   // of one KV head's rows in a page
+    float* part;           // [workgroup][16][head size]: unnormalised outputs
+    float* part_ml;        // [workgroup][16]: (max in log2 units, sum)
+    uint32_t* tickets;     // [request][KV head], kTicketStride words apart
 };
 
 // Request i as the device finds it.
@@ -99,6 +112,63 @@ __device__ inline uint64_t key_row(const RaggedParams& p, uint32_t request, uint
     }
 }
 
+// One query row by one wave, each product and sum in f32 and only of the keys
+// that the row sees: for rows whose output a tile of the kernels below leaves
+// non-finite, where 0 * inf and 0 * NaN of keys behind a row, or a page outside
+// the pool, may have reached it.  Lane = key for the scores, lane = elements
+// lane + 64 e for the values.  Head sizes up to 128, elements aligned to
+// themselves.
+template <typename T, bool PAGED>
+__device__ inline void row_by_wave(const T* __restrict__ q, const T* __restrict__ k,
+                                   const T* __restrict__ v, T* __restrict__ out,
+                                   const RaggedParams& p, uint32_t request, const Request& r,
+                                   uint32_t j, uint32_t head) {
+    const uint32_t lane = threadIdx.x % 64, D = p.head_dim, kv_head = head / p.group;
+    const T* qrow = q + (r.begin + j) * p.q_token + head * p.q_head;
+    const int64_t position = r.first + j;
+    const uint32_t key_end = position < 0 ? 0u : uint32_t(position) + 1;
+    float o[2] = {0.0f, 0.0f}, m = -INFINITY, l = 0.0f;
+    for (uint32_t base = 0; base < key_end; base += 64) {
+        const uint32_t n = min(64u, key_end - base);
+        const uint32_t key = base + min(lane, n - 1);
+        const uint64_t krow =
+            key_row<PAGED>(p, request, r.begin, key, kv_head, p.k_token, p.k_head);
+        float s = krow == kNoRow ? NAN : 0.0f;
+        if (krow != kNoRow) {
+            for (uint32_t d = 0; d < D; ++d)
+                s = __builtin_fmaf(to_float(qrow[d]), to_float(k[krow + d]), s);
+            s *= p.scale;
+        }
+        if (lane >= n) s = -INFINITY;
+        const float m_new = fmaxf(m, wave_max_dpp(s));
+        const float shift = m_new == -INFINITY ? 0.0f : m_new;
+        const float alpha = exp_fast(m - shift), e = exp_fast(s - shift);
+        m = m_new;
+        l = l * alpha + e;
+        o[0] *= alpha;
+        o[1] *= alpha;
+        for (uint32_t i = 0; i < n; ++i) {
+            const float pi = lane_value(e, int(i));
+            const uint64_t vrow =
+                key_row<PAGED>(p, request, r.begin, base + i, kv_head, p.v_token, p.v_head);
+#pragma unroll
+            for (int e2 = 0; e2 < 2; ++e2) {
+                const uint32_t d = lane + 64 * e2;
+                const bool there = vrow != kNoRow && d < D;
+                o[e2] += pi * (there ? to_float(v[vrow + d]) : 0.0f);
+            }
+        }
+    }
+    l = wave_sum_dpp(l);
+    const float inv = r.bad ? NAN : key_end == 0 ? 0.0f : 1.0f / l;
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+        const uint32_t d = lane + 64 * e;
+        if (d < D)
+            out[(uint64_t(r.begin + j) * p.q_heads + head) * D + d] = from_float<T>(o[e] * inv);
+    }
+}
+
 // ------------------------------------------------- one wave per query row
 //
 // Any head size up to 512, any strides and alignment: keys 256 at a time, a
@@ -118,7 +188,7 @@ __global__ __launch_bounds__(64) void k_ragged_rows(const T* __restrict__ q,
     const uint32_t t = blockIdx.x / p.q_heads, head = blockIdx.x % p.q_heads;
     const uint32_t i = find_request(p, t);
     const Request r = load_request<PAGED>(p, i);
-    if (t < r.begin || t - r.begin >= r.n) return;
+    if (t < r.begin || t - r.begin >= r.n || r.n * p.group <= p.small_rows) return;
     const uint32_t D = p.head_dim, kv_head = head / p.group;
     const int64_t position = r.first + (t - r.begin);
     const uint32_t key_end = position < 0 ? 0u : uint32_t(position) + 1;
@@ -189,14 +259,472 @@ __global__ __launch_bounds__(64) void k_ragged_rows(const T* __restrict__ q,
     }
 }
 
+// ------------------------------------------- few rows per KV head (decode)
+//
+// The rows of a request that share a KV head (tokens times group, row r = token
+// r / group, head r % group) are the 16 columns of one matrix tile, and its
+// keys stream past them once: S^T = K Q^T, P = 2^(S scale log2 e - max), O^T +=
+// V^T P^T, per wave in its own registers.
+//
+// Work: every request's keys are cut into units of 4 kKeys (one block of kKeys
+// for each of a workgroup's four waves), and the units of all requests into
+// ranges of the same count, one a workgroup, no range over two requests.  The
+// lengths are only here, so every workgroup finds its range itself: a wave sums
+// the units over the requests, which gives the count per range, and a second
+// sum gives its request.  Partials of a request in several ranges meet by a
+// ticket: the workgroup that finishes last merges them.
+//
+// Layout: K's operand is its rows as they lie in memory (16 bytes a lane).  V's
+// has to come by columns: a lane loads its 4 or 8 columns of eight
+// neighbouring rows (f32: of four) and takes the operand of each column across
+// those registers (v_perm), so nothing passes through LDS.  Rows of the score
+// tiles are keys in the order that leaves a lane the probabilities of exactly
+// those eight rows.  The next block's K and V are in flight while one is
+// computed, and the page entries one block further ahead.  Bound by HBM.
+template <typename T, int DP>
+struct SplitShape {
+    static constexpr bool kHalf = std::is_same<T, half_t>::value;
+    static constexpr int kKeys = (kHalf ? 4096 : 2048) / DP;  // keys of a block
+    static constexpr int kKTiles = kKeys / 16;
+    static constexpr int kKChunks = kHalf ? DP / 32 : DP / 16;  // 16-byte pieces of a K row a lane
+    static constexpr int kVRows = kHalf ? 8 : 4;                // neighbouring V rows a lane
+    static constexpr int kVSteps = kKeys / (4 * kVRows);
+    static constexpr int kVCols = kHalf ? DP / 16 : 4;          // columns of one V load
+    static constexpr int kVChunks = kHalf ? 1 : DP / 64;
+    static constexpr int kTiles = DP / 16;                      // 16-element tiles of the output
+};
+typedef half_t hv4 __attribute__((ext_vector_type(4)));
+
+template <typename T, int DP>
+struct SplitBlock {
+    typedef SplitShape<T, DP> S;
+    typedef typename std::conditional<S::kHalf, h8, f32x4>::type KV;
+    typedef typename std::conditional<S::kHalf, typename VecOf<half_t, DP / 16>::type,
+                                      f32x4>::type VV;
+    KV k[S::kKTiles][S::kKChunks];
+    VV v[S::kVSteps][S::kVRows][S::kVChunks];
+};
+
+constexpr uint32_t kSplitRows = 16;
+constexpr int kSplitWaves = 4;
+constexpr uint32_t kTicketStride = 64;
+
+__device__ inline float columns_max(float v) {  // over lanes l, l ^ 16, l ^ 32, l ^ 48
+    auto s = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    v = fmaxf(__uint_as_float(s[0]), __uint_as_float(s[1]));
+    s = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return fmaxf(__uint_as_float(s[0]), __uint_as_float(s[1]));
+}
+__device__ inline float columns_sum(float v) {
+    auto s = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    v = __uint_as_float(s[0]) + __uint_as_float(s[1]);
+    s = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return __uint_as_float(s[0]) + __uint_as_float(s[1]);
+}
+
+// Agent-coherent pairs of floats: written through, and read past, an XCD's L2.
+__device__ inline void publish2(float* p, float a, float b) {
+    const uint64_t w = uint64_t(__float_as_uint(a)) | uint64_t(__float_as_uint(b)) << 32;
+    __hip_atomic_store(reinterpret_cast<uint64_t*>(p), w, __ATOMIC_RELAXED,
+                       __HIP_MEMORY_SCOPE_AGENT);
+}
+__device__ inline float2 observe2(const float* p) {
+    const uint64_t w = __hip_atomic_load(reinterpret_cast<const uint64_t*>(p), __ATOMIC_RELAXED,
+                                         __HIP_MEMORY_SCOPE_AGENT);
+    return make_float2(__uint_as_float(uint32_t(w)), __uint_as_float(uint32_t(w >> 32)));
+}
+
+// A request's units for the split kernel, 0 if it is not one of its own.
+__device__ inline uint32_t split_units(const RaggedParams& p, uint32_t i, uint32_t unit_shift) {
+    if (i >= p.sequences) return 0u;
+    const Request r = load_request<true>(p, i);
+    if (r.n == 0 || r.n * p.group > p.small_rows) return 0u;
+    // no keys to read where every row is zero or NaN: one unit writes them
+    const uint32_t units = uint32_t((uint64_t(r.keys) + (1u << unit_shift) - 1) >> unit_shift);
+    return r.bad || units == 0 ? 1u : units;
+}
+
+__device__ inline uint32_t wave_scan(uint32_t v) {  // inclusive sum
+    v += uint32_t(__builtin_amdgcn_update_dpp(0, int(v), 0x111, 0xF, 0xF, false));
+    v += uint32_t(__builtin_amdgcn_update_dpp(0, int(v), 0x112, 0xF, 0xF, false));
+    v += uint32_t(__builtin_amdgcn_update_dpp(0, int(v), 0x114, 0xF, 0xF, false));
+    v += uint32_t(__builtin_amdgcn_update_dpp(0, int(v), 0x118, 0xF, 0xF, false));
+    v += uint32_t(__builtin_amdgcn_update_dpp(0, int(v), 0x142, 0xA, 0xF, false));
+    v += uint32_t(__builtin_amdgcn_update_dpp(0, int(v), 0x143, 0xC, 0xF, false));
+    return v;
+}
+__device__ inline uint32_t last_lane(uint32_t v) {
+    return uint32_t(__builtin_amdgcn_readlane(int(v), 63));
+}
+
+// FULL: the head size is DP; else it is a smaller multiple of 16 bytes and the
+// operands' elements past it are zeros (K, Q) or any row's own (V, whose output
+// columns are not stored).
+template <typename T, int DP, bool FULL>
+__global__ __launch_bounds__(64 * kSplitWaves, 2) void k_ragged_split(
+    const T* __restrict__ q, const T* __restrict__ k, const T* __restrict__ v,
+    T* __restrict__ out, RaggedParams p) {
+    typedef SplitShape<T, DP> S;
+    typedef SplitBlock<T, DP> Block;
+    typedef typename Block::KV KV;
+    typedef typename Block::VV VV;
+    constexpr bool kHalf = S::kHalf;
+    constexpr uint32_t kKeys = S::kKeys;
+    constexpr uint32_t kUnit = kSplitWaves * kKeys;
+    constexpr uint32_t kUnitShift = __builtin_ctz(kUnit);
+    __shared__ float merge_ml[kSplitWaves][kSplitRows][2];
+    __shared__ __align__(16) float merge_o[kSplitWaves][kSplitRows][DP + 4];
+    __shared__ uint32_t odd_rows, ticket;
+    const uint32_t hd = FULL ? uint32_t(DP) : p.head_dim;
+    const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
+    const uint32_t lane = threadIdx.x % 64;
+    const uint32_t lr = lane % 16, g = lane / 16;
+    const uint32_t kvh = blockIdx.x % p.kv_heads, w = blockIdx.x / p.kv_heads;
+
+    // this workgroup's request and key range
+    const uint32_t units0 = split_units(p, lane, kUnitShift);  // of the first 64 requests
+    uint64_t total = last_lane(wave_scan(units0));
+    for (uint32_t base = 64; base < p.sequences; base += 64)
+        total += last_lane(wave_scan(split_units(p, base + lane, kUnitShift)));
+    const uint32_t per = max(1u, uint32_t((total + p.share - 1) / p.share));
+    uint32_t before = 0, request = p.sequences, first_split = 0, n_splits = 0;
+    for (uint32_t base = 0; base < p.sequences; base += 64) {
+        const uint32_t units = base == 0 ? units0 : split_units(p, base + lane, kUnitShift);
+        const uint32_t mine = (units + per - 1) / per;
+        const uint32_t upto = before + wave_scan(mine);
+        const uint64_t past = __ballot(upto > w);
+        if (past != 0) {
+            const int at = __builtin_ctzll(past);
+            request = base + at;
+            n_splits = uint32_t(__builtin_amdgcn_readlane(int(mine), at));
+            first_split = uint32_t(__builtin_amdgcn_readlane(int(upto), at)) - n_splits;
+            break;
+        }
+        before = last_lane(upto);
+    }
+    if (request >= p.sequences) return;  // more workgroups than ranges
+    const Request r = load_request<true>(p, request);
+    const uint32_t split = w - first_split;
+    const uint32_t R = r.n * p.group;
+    const uint32_t last = r.keys == 0 ? 0u : r.keys - 1;
+    const uint32_t blocks = r.bad ? 0u : (r.keys + kKeys - 1) / kKeys;
+    const uint32_t b0 = split * per * kSplitWaves;
+    const uint32_t b1 = min(blocks, b0 + per * kSplitWaves);
+
+    const uint32_t* entries = p.table + uint64_t(request) * p.max_blocks;
+    bool bad_page = false;
+    auto load_entry = [&](uint32_t blk) {  // of key blk * kKeys + lane
+        const uint32_t key = min(blk * kKeys + lane % kKeys, last);
+        return entries[key >> p.shift];
+    };
+    auto checked = [&](uint32_t entry) {  // a page outside the pool: page 0 instead, and noted
+        bad_page |= entry >= p.pages;
+        return entry < p.pages ? entry : 0u;
+    };
+    const uint32_t mask = (1u << p.shift) - 1;
+    const uint32_t row_bytes = hd * sizeof(T);
+    const char* kbase = reinterpret_cast<const char*>(k) + uint64_t(kvh) * p.head_bytes + 16 * g;
+    // columns kVCols lr .. of V, those past the head size read the first ones
+    const uint32_t col = S::kVCols * lr;
+    const char* vbase = reinterpret_cast<const char*>(v) + uint64_t(kvh) * p.head_bytes;
+    auto load_block = [&](Block& x, uint32_t blk, uint32_t entry) {
+        const uint32_t kb = blk * kKeys;
+#pragma unroll
+        for (int m = 0; m < S::kKTiles; ++m) {
+            const uint32_t kk = kHalf ? 32 * (m / 2) + 8 * (lr / 4) + 4 * (m % 2) + lr % 4
+                                      : 16 * m + lr;
+            const uint32_t key = min(kb + kk, last);
+            const uint32_t page = uint32_t(__shfl(int(entry), int(key - kb), 64));
+            const char* row = kbase + uint64_t(page) * p.page_bytes + (key & mask) * row_bytes;
+#pragma unroll
+            for (int c = 0; c < S::kKChunks; ++c) {
+                const bool in = FULL || uint32_t(64 * c) + 16 * g < row_bytes;
+                x.k[m][c] = in ? *reinterpret_cast<const KV*>(row + 64 * c) : KV{};
+            }
+        }
+#pragma unroll
+        for (int t = 0; t < S::kVSteps; ++t) {
+            const uint32_t run = kb + 4 * S::kVRows * t + S::kVRows * g;  // inside one page
+            const uint32_t page =
+                uint32_t(__shfl(int(entry), int(min(run, last) - kb), 64));
+            const char* rows = vbase + uint64_t(page) * p.page_bytes;
+#pragma unroll
+            for (int e = 0; e < S::kVRows; ++e) {
+                const char* row = rows + (min(run + e, last) & mask) * row_bytes;
+#pragma unroll
+                for (int c = 0; c < S::kVChunks; ++c) {
+                    const uint32_t at = col + 64 * c;
+                    x.v[t][e][c] = *reinterpret_cast<const VV*>(
+                        row + sizeof(T) * (FULL || at < hd ? at : 0u));
+                }
+            }
+        }
+    };
+
+    // row lr of this KV head: query elements, last key it sees (-1: none)
+    const bool row_live = lr < R;
+    const uint32_t token = row_live ? lr / p.group : 0u, sub = row_live ? lr % p.group : 0u;
+    const int64_t position = r.first + token;
+    const int limit = row_live && position >= 0 ? int(min(int64_t(last), position)) : -1;
+    const T* qrow = q + (r.begin + token) * p.q_token + (kvh * p.group + sub) * p.q_head;
+    KV qf[S::kKChunks];
+#pragma unroll
+    for (int c = 0; c < S::kKChunks; ++c) {
+        const bool in = FULL || uint32_t(64 * c) + 16 * g < row_bytes;
+        qf[c] = in ? *reinterpret_cast<const KV*>(reinterpret_cast<const char*>(qrow) + 16 * g +
+                                                  64 * c)
+                   : KV{};
+    }
+    f32x4 o[S::kTiles];
+#pragma unroll
+    for (int t = 0; t < S::kTiles; ++t) o[t] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    float m = -INFINITY, l = 0.0f;  // l: this lane's share
+
+    auto compute = [&](const Block& x, uint32_t blk) {
+        f32x4 s[S::kKTiles];
+#pragma unroll
+        for (int t = 0; t < S::kKTiles; ++t) {
+            s[t] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+            for (int c = 0; c < S::kKChunks; ++c) {
+                if constexpr (kHalf) {
+                    s[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(x.k[t][c], qf[c], s[t], 0, 0, 0);
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        s[t] = __builtin_amdgcn_mfma_f32_16x16x4f32(x.k[t][c][e], qf[c][e], s[t],
+                                                                    0, 0, 0);
+                }
+            }
+        }
+        // register r of tile t: key blk kKeys + (a constant) + 8 g (f32: 4 g)
+        const int seen = limit - int(blk * kKeys) - int(S::kVRows * g);
+        float mx = -INFINITY;
+#pragma unroll
+        for (int t = 0; t < S::kKTiles; ++t)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const int at = kHalf ? 32 * (t / 2) + 4 * (t % 2) + e : 16 * t + e;
+                s[t][e] = at <= seen ? s[t][e] : -INFINITY;
+                mx = fmaxf(mx, s[t][e]);
+            }
+        mx = columns_max(mx) * p.scale_log2;
+        const float m_new = fmaxf(m, mx);
+        const float shift = m_new == -INFINITY ? 0.0f : m_new;
+        const float alpha = __builtin_amdgcn_exp2f(m - shift);
+        m = m_new;
+        l *= alpha;
+#pragma unroll
+        for (int t = 0; t < S::kTiles; ++t)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o[t][e] *= alpha;
+#pragma unroll
+        for (int t = 0; t < S::kKTiles; ++t)
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                s[t][e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[t][e], p.scale_log2, -shift));
+        if constexpr (kHalf) {
+#pragma unroll
+            for (int t = 0; t < S::kVSteps; ++t) {
+                h8 pb;
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    pb[e] = half_t(s[2 * t + e / 4][e % 4]);
+                    l += float(pb[e]);  // the sum of the rounded ones, as the product takes them
+                }
+#pragma unroll
+                for (int c = 0; c < S::kTiles; ++c) {
+                    h8 va;
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) va[e] = x.v[t][e][0][c];
+                    o[c] = __builtin_amdgcn_mfma_f32_16x16x32_f16(va, pb, o[c], 0, 0, 0);
+                }
+            }
+        } else {
+#pragma unroll
+            for (int t = 0; t < S::kVSteps; ++t)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    l += s[t][e];
+#pragma unroll
+                    for (int c = 0; c < S::kTiles; ++c)
+                        o[c] = __builtin_amdgcn_mfma_f32_16x16x4f32(x.v[t][e][c / 4][c % 4],
+                                                                    s[t][e], o[c], 0, 0, 0);
+                }
+        }
+    };
+
+    uint32_t blk = b0 + wave;
+    if (blk < b1) {
+        Block a, b;
+        uint32_t entry = load_entry(blk);
+        uint32_t ahead = load_entry(min(blk + kSplitWaves, b1 - 1));
+        load_block(a, blk, checked(entry));
+        while (true) {
+            if (blk + kSplitWaves >= b1) {
+                compute(a, blk);
+                break;
+            }
+            entry = ahead;
+            ahead = load_entry(min(blk + 2 * kSplitWaves, b1 - 1));
+            load_block(b, blk + kSplitWaves, checked(entry));
+            compute(a, blk);
+            blk += kSplitWaves;
+            if (blk + kSplitWaves >= b1) {
+                compute(b, blk);
+                break;
+            }
+            entry = ahead;
+            ahead = load_entry(min(blk + 2 * kSplitWaves, b1 - 1));
+            load_block(a, blk + kSplitWaves, checked(entry));
+            compute(b, blk);
+            blk += kSplitWaves;
+        }
+    }
+    l = columns_sum(l);
+    if (__any(bad_page)) l = NAN;  // row_by_wave finds which rows see it
+
+    // the four waves' states -> the range's.  Lane (g, lr), f16: elements
+    // kTiles (4 g + e) + c of row lr in o[c][e]; f32: 64 (c / 4) + 4 (4 g + e) + c % 4.
+    if (threadIdx.x == 0) odd_rows = 0;
+    if (g == 0) {
+        merge_ml[wave][lr][0] = m;
+        merge_ml[wave][lr][1] = l;
+    }
+#pragma unroll
+    for (int c = 0; c < S::kTiles; ++c)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const uint32_t at =
+                kHalf ? S::kTiles * (4 * g + e) + c : 64 * (c / 4) + 4 * (4 * g + e) + c % 4;
+            merge_o[wave][lr][at] = o[c][e];
+        }
+    __syncthreads();
+    const uint32_t slot = kvh * p.splits + w;
+    const uint32_t pairs = hd / 2;
+    // row `row`'s output, two elements: stored unless it is not finite
+    auto store_row = [&](uint32_t row, uint32_t d, float2 x, float sum) {
+        const uint32_t tok = row / p.group;
+        const int64_t pos = r.first + tok;
+        const float inv = pos < 0 ? 0.0f : 1.0f / sum;
+        x.x *= inv;
+        x.y *= inv;
+        if (r.bad) x = make_float2(NAN, NAN);
+        else if (!(fabsf(x.x) < INFINITY && fabsf(x.y) < INFINITY)) atomicOr(&odd_rows, 1u << row);
+        T* dst = out + (uint64_t(r.begin + tok) * p.q_heads + kvh * p.group + row % p.group) * hd + d;
+        dst[0] = from_float<T>(x.x);
+        dst[1] = from_float<T>(x.y);
+    };
+    for (uint32_t i = threadIdx.x; i < R * pairs; i += 64 * kSplitWaves) {
+        const uint32_t row = i / pairs, d = 2 * (i % pairs);
+        float top = -INFINITY;
+#pragma unroll
+        for (int x = 0; x < kSplitWaves; ++x) top = fmaxf(top, merge_ml[x][row][0]);
+        const float shift = top == -INFINITY ? 0.0f : top;
+        float sum = 0.0f;
+        float2 acc = make_float2(0.0f, 0.0f);
+#pragma unroll
+        for (int x = 0; x < kSplitWaves; ++x) {
+            const float f = __builtin_amdgcn_exp2f(merge_ml[x][row][0] - shift);
+            sum += f * merge_ml[x][row][1];
+            acc.x += f * merge_o[x][row][d];
+            acc.y += f * merge_o[x][row][d + 1];
+        }
+        if (n_splits == 1) {
+            store_row(row, d, acc, sum);
+        } else {
+            publish2(p.part + (uint64_t(slot) * kSplitRows + row) * DP + d, acc.x, acc.y);
+            if (d == 0) publish2(p.part_ml + (uint64_t(slot) * kSplitRows + row) * 2, top, sum);
+        }
+    }
+    if (n_splits > 1) {
+        // Hand-over: every wave's published stores are complete (they are
+        // written through to where all XCDs see them, and vmcnt 0 waits for
+        // that) before the barrier, and only then is the ticket drawn; the
+        // workgroup that draws the last one acquires and reads past its L2.
+        // As for the decode of rl_attention_*, the order of the stores and the
+        // ticket rests on that wait, not on a release, which would write back
+        // the whole L2 in every workgroup.
+        __builtin_amdgcn_s_waitcnt(0);
+        __syncthreads();
+        uint32_t* counter = p.tickets + (uint64_t(request) * p.kv_heads + kvh) * kTicketStride;
+        if (threadIdx.x == 0)
+            ticket = __hip_atomic_fetch_add(counter, 1u, __ATOMIC_RELAXED,
+                                            __HIP_MEMORY_SCOPE_AGENT);
+        __syncthreads();
+        if (ticket != n_splits - 1) return;
+        __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "agent");
+        if (threadIdx.x == 0)  // for the next call
+            __hip_atomic_store(counter, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        constexpr uint32_t kChunk = 8;
+        const uint64_t slot0 = uint64_t(kvh) * p.splits + first_split;
+        for (uint32_t i = threadIdx.x; i < R * pairs; i += 64 * kSplitWaves) {
+            const uint32_t row = i / pairs, d = 2 * (i % pairs);
+            float top = -INFINITY, sum = 0.0f;
+            float2 acc = make_float2(0.0f, 0.0f);
+            for (uint32_t s0 = 0; s0 < n_splits; s0 += kChunk) {
+                float2 ml[kChunk], ov[kChunk];
+#pragma unroll
+                for (uint32_t x = 0; x < kChunk; ++x) {
+                    const uint64_t at =
+                        (slot0 + min(s0 + x, n_splits - 1)) * kSplitRows + row;
+                    ml[x] = observe2(p.part_ml + at * 2);
+                    ov[x] = observe2(p.part + at * DP + d);
+                }
+                float next = top;
+#pragma unroll
+                for (uint32_t x = 0; x < kChunk; ++x)
+                    if (s0 + x < n_splits) next = fmaxf(next, ml[x].x);
+                const float shift = next == -INFINITY ? 0.0f : next;
+                const float keep = __builtin_amdgcn_exp2f(top - shift);
+                sum *= keep;
+                acc.x *= keep;
+                acc.y *= keep;
+#pragma unroll
+                for (uint32_t x = 0; x < kChunk; ++x) {
+                    if (s0 + x >= n_splits) continue;
+                    const float f = __builtin_amdgcn_exp2f(ml[x].x - shift);
+                    sum += f * ml[x].y;
+                    acc.x += f * ov[x].x;
+                    acc.y += f * ov[x].y;
+                }
+                top = next;
+            }
+            store_row(row, d, acc, sum);
+        }
+    }
+    // rows with an output that is not finite once more (after the stores above)
+    __builtin_amdgcn_s_waitcnt(0);
+    __syncthreads();
+    uint32_t odd = odd_rows;
+    for (uint32_t n = 0; odd != 0; odd &= odd - 1, ++n) {
+        if (n % kSplitWaves != wave) continue;
+        const uint32_t row = __builtin_ctz(odd);
+        row_by_wave<T, true>(q, k, v, out, p, request, r, row / p.group,
+                             kvh * p.group + row % p.group);
+    }
+}
+
 // -------------------------------------------------------------- workspace
+//
+// The split kernel's partials and tickets.  Its workgroups a KV head: `share`
+// equal ranges of all units, and up to one more a request for the ranges that
+// end with it.  Ranges are counted for two workgroups a CU, its registers'
+// occupancy; several requests of different lengths leave short last ranges, so
+// they are cut finer.
+struct WorkspaceNeed {
+    uint64_t share, splits;
+    rl_context::Workspace size;
+};
 
-constexpr uint64_t kWorkspaceAlign = 256;
-
-uint64_t workspace_bytes(const rl_context* ctx, uint64_t sequences, uint64_t tokens,
-                         uint64_t q_heads, uint64_t kv_heads, uint64_t head_dim) {
-    (void)ctx, (void)sequences, (void)tokens, (void)q_heads, (void)kv_heads, (void)head_dim;
-    return kWorkspaceAlign;
+WorkspaceNeed workspace_for(const rl_context* ctx, uint64_t sequences, uint64_t kv_heads) {
+    WorkspaceNeed w{};
+    const uint64_t rounds = sequences == 1 ? 1 : sequences < 4 ? 2 : 4;
+    w.share = ceil_div(rounds * 2 * uint64_t(ctx->num_cus), kv_heads);
+    w.splits = w.share + sequences;
+    w.size.ticket_bytes = sequences * kv_heads * kTicketStride * sizeof(uint32_t);
+    w.size.partial_bytes = w.splits * kv_heads * kSplitRows * (128 + 2) * sizeof(float);
+    return w;
 }
 
 // ------------------------------------------------------------- validation
@@ -233,6 +761,20 @@ void launch_rows(rl_context* ctx, const T* q, const T* k, const T* v, T* out,
         RL_LAUNCH(ctx, (k_ragged_rows<T, 4, PAGED>), grid, block, q, k, v, out, p);
     else
         RL_LAUNCH(ctx, (k_ragged_rows<T, 8, PAGED>), grid, block, q, k, v, out, p);
+}
+
+template <typename T>
+void launch_split(rl_context* ctx, const T* q, const T* k, const T* v, T* out,
+                  const RaggedParams& p) {
+    const dim3 grid(p.splits * p.kv_heads), block(64 * kSplitWaves);
+    if (p.head_dim == 64)
+        RL_LAUNCH(ctx, (k_ragged_split<T, 64, true>), grid, block, q, k, v, out, p);
+    else if (p.head_dim < 64)
+        RL_LAUNCH(ctx, (k_ragged_split<T, 64, false>), grid, block, q, k, v, out, p);
+    else if (p.head_dim == 128)
+        RL_LAUNCH(ctx, (k_ragged_split<T, 128, true>), grid, block, q, k, v, out, p);
+    else
+        RL_LAUNCH(ctx, (k_ragged_split<T, 128, false>), grid, block, q, k, v, out, p);
 }
 
 template <typename T>
@@ -319,14 +861,19 @@ rl_status paged_entry(rl_context* ctx, const char* name, const rl_buffer* q,
     if (rl_status st = check_output(out, numel, es, "paged attention")) return st;
     if (rl_status st = check_buffer(workspace, "workspace")) return st;
     if (rl_status st = require_context(ctx)) return st;
-    const uint64_t need = workspace_bytes(ctx, sequences, tokens, q_heads, kv_heads, head_dim);
-    if (ctx->workspaces.count(workspace->data) == 0)
+    const WorkspaceNeed w = workspace_for(ctx, sequences, kv_heads);
+    const auto held = ctx->workspaces.find(workspace->data);
+    if (held == ctx->workspaces.end())
         return fail(RL_ERR_INVALID_ARGUMENT,
                     "the workspace is not one of rl_paged_attention_workspace on this context");
-    if (ctx->workspaces[workspace->data] < need)
-        return fail(RL_ERR_INVALID_SHAPE, "workspace has %llu bytes, expected %llu",
-                    (unsigned long long)ctx->workspaces[workspace->data],
-                    (unsigned long long)need);
+    if (held->second.ticket_bytes < w.size.ticket_bytes ||
+        held->second.partial_bytes < w.size.partial_bytes)
+        return fail(RL_ERR_INVALID_SHAPE,
+                    "the workspace holds %llu + %llu bytes, expected %llu + %llu",
+                    (unsigned long long)held->second.ticket_bytes,
+                    (unsigned long long)held->second.partial_bytes,
+                    (unsigned long long)w.size.ticket_bytes,
+                    (unsigned long long)w.size.partial_bytes);
     if (rl_status st = activate(ctx)) return st;
 
     RaggedParams p{};
@@ -348,9 +895,31 @@ rl_status paged_entry(rl_context* ctx, const char* name, const rl_buffer* q,
     p.q_head = head_dim;
     p.scale = scale;
     p.scale_log2 = scale * kLog2e;
-    launch_rows<T, true>(ctx, static_cast<const T*>(q->data),
-                         static_cast<const T*>(k_pages->data),
-                         static_cast<const T*>(v_pages->data), static_cast<T*>(out->data), p);
+    const T* qd = static_cast<const T*>(q->data);
+    const T* kd = static_cast<const T*>(k_pages->data);
+    const T* vd = static_cast<const T*>(v_pages->data);
+    T* od = static_cast<T*>(out->data);
+    // the matrix-core kernels: rows of whole 16-byte pieces up to 128 elements,
+    // pages of at least the eight rows a lane's value loads take from one
+    const uint64_t page_bytes = kv_heads * page_size * head_dim * es;
+    const bool matrix = head_dim * es % 16 == 0 && head_dim <= 128 && page_size >= 8 &&
+                        page_bytes <= UINT32_MAX && aligned_to(qd, 16) && aligned_to(kd, 16) &&
+                        aligned_to(vd, 16);
+    const uint64_t most_rows = std::min(max_queries, tokens) * p.group;
+    if (matrix && p.group <= kSplitRows) {
+        char* ws = static_cast<char*>(workspace->data);
+        p.small_rows = kSplitRows;
+        p.share = uint32_t(w.share);
+        p.splits = uint32_t(w.splits);
+        p.page_bytes = uint32_t(page_bytes);
+        p.head_bytes = uint32_t(page_size * head_dim * es);
+        p.tickets = reinterpret_cast<uint32_t*>(ws);
+        p.part = reinterpret_cast<float*>(ws + held->second.ticket_bytes);
+        p.part_ml = p.part + w.splits * kv_heads * kSplitRows * 128;
+        launch_split<T>(ctx, qd, kd, vd, od, p);
+        if (most_rows <= kSplitRows) return after_launch(ctx, name);
+    }
+    launch_rows<T, true>(ctx, qd, kd, vd, od, p);
     return after_launch(ctx, name);
 }
 
@@ -363,15 +932,16 @@ rl_status workspace_entry(rl_context* ctx, uint64_t sequences, uint64_t tokens, 
     if (rl_status st = require_context(ctx)) return st;
     if (ctx->capturing)
         return fail(RL_ERR_DEVICE, "a workspace cannot be made while recording a graph");
-    const uint64_t bytes = workspace_bytes(ctx, sequences, tokens, q_heads, kv_heads, head_dim);
+    const rl_context::Workspace size = workspace_for(ctx, sequences, kv_heads).size;
+    const uint64_t bytes = size.ticket_bytes + size.partial_bytes;
     rl_buffer made{nullptr, 0, 0};
     if (rl_status st = rl_buffer_empty(ctx, bytes, 1, &made)) return st;
-    const hipError_t err = hipMemsetAsync(made.data, 0, bytes, ctx->stream);
+    const hipError_t err = hipMemsetAsync(made.data, 0, size.ticket_bytes, ctx->stream);
     if (err != hipSuccess) {
         rl_buffer_release(ctx, &made);
         return fail(RL_ERR_DEVICE, "workspace: %s", hipGetErrorString(err));
     }
-    ctx->workspaces[made.data] = bytes;
+    ctx->workspaces[made.data] = size;
     *out = made;
     return RL_OK;
 }
