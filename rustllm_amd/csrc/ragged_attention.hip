@@ -705,6 +705,470 @@ __global__ __launch_bounds__(64 * kSplitWaves, 2) void k_ragged_split(
     }
 }
 
+// -------------------------------------------------- many rows per KV head
+//
+// A tile is 32 QW of the rows that share a KV head (row r = token r / group,
+// head r % group of the KV head's): every K and V block serves all heads of the
+// group, and a causal tile is no longer than its 32 QW / group tokens.  Four
+// waves: QW of 32 rows times KS shares of the key blocks, merged through LDS at
+// the end.  S^T = K Q^T leaves each lane one row's scores (32 x 32 tiles), so
+// the running max and sum need one exchange between lane halves, and the
+// probabilities come out in the operand layout of O^T += V^T P^T: for f16 with
+// keys taken in perm32 order, V's operand by transpose reads out of LDS; for
+// f32 (32x32x2 products) as they stand, V read by rows, lane i of a half
+// holding elements EC i .. + EC - 1 of it.
+// K and V go from memory straight to LDS (two stages), each lane fetching 16
+// bytes from an address of its own -- its key's row, wherever its page is --
+// the page entries read a step ahead.  Keys past the request's last read that
+// last row again: nothing outside the request's rows is read, and their scores
+// are masked.  Chunk c of row r lies at c ^ lds_swizzle(r).
+//
+// Tiles are numbered without a sum over the requests: request i's first tile is
+// floor(o_i group / TILE) + i, which leaves room for all of its tiles.  Later
+// tiles, the longer ones, start first; neighbouring workgroups take
+// different KV heads, so that one XCD's workgroups (every eighth) share rows of
+// K and V in its L2.
+template <int QW>
+constexpr uint32_t kTileRows = 32 * QW;
+
+// One 16-byte chunk a lane from memory to LDS: lane l's lands at lds + 16 l.
+// In assembly so that the compiler's wait counting does not hold the LDS reads
+// of the stage in use for a stage being filled; the caller waits for it
+// (vmcnt) before the barrier that hands the stage over.
+__device__ inline void load_to_lds(const void* from, uint32_t lds) {
+    uint32_t saved;
+    asm volatile(
+        "s_mov_b32 %0, m0\n\t"
+        "s_mov_b32 m0, %1\n\t"
+        "s_nop 0\n\t"
+        "global_load_lds_dwordx4 %2, off\n\t"
+        "s_mov_b32 m0, %0"
+        : "=&s"(saved)
+        : "s"(lds), "v"(from)
+        : "memory");
+}
+
+// max over lanes l and l ^ 32
+__device__ inline float halves_max(float v) {
+    const auto s = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false,
+                                                    false);
+    return fmaxf(__uint_as_float(s[0]), __uint_as_float(s[1]));
+}
+// max(a, b, c) as one instruction (fmaxf would first canonicalise what comes
+// out of a matrix product)
+__device__ inline float max3(float a, float b, float c) {
+    float r;
+    asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "v"(c));
+    return r;
+}
+
+// Zeros for the chunks of a padded K row.
+__device__ __align__(16) const uint32_t zero_chunk[4] = {0, 0, 0, 0};
+
+// A row's running max (log2 units) moves only when a block passes it by more
+// than this: probabilities stay below 2^3, and most blocks skip the rescaling.
+constexpr float kSlack = 3.0f;
+
+// Tile u's request: the last one whose first tile is not past u (64 candidates
+// a step).
+__device__ inline uint32_t tiles_before(const RaggedParams& p, uint32_t i, uint32_t rows) {
+    return uint32_t(uint64_t(min(p.offsets[i], p.tokens)) * p.group / rows) + i;
+}
+__device__ inline uint32_t find_tile_request(const RaggedParams& p, uint32_t u, uint32_t rows) {
+    const uint32_t lane = threadIdx.x % 64;
+    uint32_t lo = 0, hi = p.sequences;
+    while (hi - lo > 1) {
+        const uint32_t step = (hi - lo + 63) / 64;
+        const uint64_t at = lo + uint64_t(lane) * step;
+        const bool ok = at < hi && tiles_before(p, uint32_t(at), rows) <= u;
+        const uint64_t found = __ballot(ok);
+        const uint32_t k = found == 0 ? 0u : 63u - uint32_t(__builtin_clzll(found));
+        lo += k * step;
+        hi = min(hi, lo + step);
+    }
+    return __builtin_amdgcn_readfirstlane(lo);
+}
+
+// Waves a SIMD that the registers leave room for: two where two workgroups of
+// four waves fit a CU's LDS.
+template <typename T, int NT, int QW, int KS, int BN>
+constexpr int kTileWaves =
+    QW * KS == 4 && 2 * KS * 2 * BN * (NT == 3 ? 128 : 32 * NT) * int(sizeof(T)) <= 72 * 1024 ? 2 : 1;
+
+template <typename T, int NT, int QW, int KS, int BN, bool PAGED, bool FULL>
+__global__ __launch_bounds__(64 * QW * KS, (kTileWaves<T, NT, QW, KS, BN>)) void k_ragged_tiles(
+    const T* __restrict__ q, const T* __restrict__ k, const T* __restrict__ v,
+    T* __restrict__ out, RaggedParams p) {
+    constexpr bool kHalf = std::is_same<T, half_t>::value;
+    constexpr int D = 32 * NT;                    // head size, padded
+    constexpr int RD = NT == 3 ? 128 : D;         // elements of an LDS row
+    constexpr int CE = 16 / int(sizeof(T));       // elements of a chunk
+    constexpr int ROW_CHUNKS = RD / CE;
+    constexpr int SW = ROW_CHUNKS >= 16 ? 4 : ROW_CHUNKS / 4;  // lds_swizzle's row class
+    constexpr int KT = BN / 32;                   // 32-key tiles of a block
+    constexpr int DC = D / (2 * CE);              // pairs of chunks of a row (lane halves)
+    constexpr int EC = D / 32;                    // f32: elements of a V row a lane
+    constexpr int WAVES = QW * KS;
+    constexpr int THREADS = 64 * WAVES;
+    constexpr uint32_t TILE = kTileRows<QW>;
+    constexpr int BLOCK_CHUNKS = BN * ROW_CHUNKS;  // of K, or V
+    constexpr int LOADS = BLOCK_CHUNKS * KS / THREADS;  // keys a lane fetches K and V chunks of
+    constexpr int BLOCK_BYTES = 16 * BLOCK_CHUNKS;
+    constexpr int STAGE_BYTES = KS * 2 * BLOCK_BYTES;
+    constexpr int MERGE = NT * 16 + 2;
+    constexpr int MERGE_BYTES = (KS - 1) * QW * 64 * MERGE * 4;
+    constexpr int LDS_BYTES = 2 * STAGE_BYTES > MERGE_BYTES ? 2 * STAGE_BYTES : MERGE_BYTES;
+    static_assert(BLOCK_CHUNKS % (64 * WAVES) == 0, "a wave's loads cover whole blocks");
+    __shared__ __align__(16) unsigned char lds[LDS_BYTES];
+    __shared__ uint32_t any_bad;
+
+    const uint32_t hd = FULL ? uint32_t(D) : p.head_dim;
+    const uint32_t kvh = blockIdx.x % p.kv_heads;
+    const uint32_t units = gridDim.x / p.kv_heads;
+    const uint32_t unit = units - 1 - blockIdx.x / p.kv_heads;
+    const uint32_t request = find_tile_request(p, unit, TILE);
+    const uint32_t tile0 = tiles_before(p, request, TILE);
+    const Request r = load_request<PAGED>(p, request);
+    const uint32_t rows = r.n * p.group;
+    const uint32_t row0 = (unit - tile0) * TILE;
+    if (unit < tile0 || row0 >= rows || rows <= p.small_rows) return;
+
+    const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
+    const uint32_t lane = threadIdx.x % 64;
+    const uint32_t qw = wave % QW, share = wave / QW;
+    const uint32_t col = lane % 32, hs = lane / 32;
+    const uint32_t last = r.keys == 0 ? 0u : r.keys - 1;
+    // keys that the tile's last row sees
+    auto keys_of = [&](uint32_t row) {  // visible to row `row` of the request
+        const int64_t pos = r.first + row / p.group;
+        return pos < 0 || r.bad ? 0u : uint32_t(min(int64_t(r.keys), pos + 1));
+    };
+    const uint32_t keys = keys_of(min(row0 + TILE, rows) - 1);
+    const uint32_t blocks = (keys + BN - 1) / BN;
+    const uint32_t steps = (blocks + KS - 1) / KS;
+    const uint32_t wrow0 = row0 + 32 * qw;  // the wave's first row
+    const bool wave_active = wrow0 < rows;
+    const uint32_t wave_keys = wave_active ? keys_of(min(wrow0 + 31, rows - 1)) : 0u;
+    const uint32_t wave_least = wave_active ? keys_of(wrow0) : 0u;  // its first row's
+    const uint32_t row = wrow0 + col;  // this lane's
+    const bool row_valid = row < rows;
+    const uint32_t token = row_valid ? row / p.group : 0u;
+    const uint32_t head = kvh * p.group + (row_valid ? row % p.group : 0u);
+    const int limit = row_valid ? int(keys_of(row)) - 1 : -1;  // last key it sees
+    if (threadIdx.x == 0) any_bad = 0;
+
+    // what a lane fetches: of key `fetch_key[i]` of its share's block, chunk `ch`
+    uint32_t fetch_key[LOADS];
+    uint32_t fetch_byte[LOADS];  // of the chunk in its row; ~0u: padding
+#pragma unroll
+    for (int i = 0; i < LOADS; ++i) {
+        // instruction i of a wave fills 64 chunks in a row of share i / PER's block
+        constexpr int PER = BLOCK_CHUNKS / (64 * WAVES);
+        const uint32_t c = ((i % PER) * WAVES + wave) * 64 + lane;  // chunk in the block
+        const uint32_t kr = c / ROW_CHUNKS;
+        const uint32_t ch = (c % ROW_CHUNKS) ^ lds_swizzle<SW>(kr);
+        fetch_key[i] = (i / PER) * BN + kr;
+        fetch_byte[i] = ch * CE < hd ? 16 * ch : ~0u;
+    }
+    const uint32_t lds_base = uint32_t(
+        reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) unsigned char*)(lds)));
+    const uint32_t* entries = PAGED ? p.table + uint64_t(request) * p.max_blocks : nullptr;
+    const uint32_t mask = (1u << p.shift) - 1;
+    const char* kbase;
+    const char* vbase;
+    if constexpr (PAGED) {
+        kbase = reinterpret_cast<const char*>(k) + uint64_t(kvh) * p.head_bytes;
+        vbase = reinterpret_cast<const char*>(v) + uint64_t(kvh) * p.head_bytes;
+    } else {
+        kbase = reinterpret_cast<const char*>(k + r.begin * p.k_token + kvh * p.k_head);
+        vbase = reinterpret_cast<const char*>(v + r.begin * p.v_token + kvh * p.v_head);
+    }
+    bool bad_page = false;
+    uint32_t entry[LOADS] = {};
+    auto load_entries = [&](uint32_t step) {
+        if constexpr (PAGED) {
+#pragma unroll
+            for (int i = 0; i < LOADS; ++i)
+                entry[i] = entries[min(step * KS * BN + fetch_key[i], last) >> p.shift];
+        }
+    };
+    auto issue_step = [&](uint32_t step) {
+        const uint32_t stage = __builtin_amdgcn_readfirstlane(
+            lds_base + (step % 2) * STAGE_BYTES + 16 * 64 * wave);
+#pragma unroll
+        for (int i = 0; i < LOADS; ++i) {
+            constexpr int PER = BLOCK_CHUNKS / (64 * WAVES);
+            if (step * KS + i / PER >= blocks) continue;
+            const uint32_t key = min(step * KS * BN + fetch_key[i], last);
+            uint64_t koff, voff;
+            if constexpr (PAGED) {
+                const bool in = entry[i] < p.pages;
+                bad_page |= !in;
+                koff = uint64_t(in ? entry[i] : 0u) * p.page_bytes +
+                       (key & mask) * uint32_t(hd * sizeof(T));
+                voff = koff;
+            } else {
+                koff = uint64_t(key) * uint32_t(p.k_token * sizeof(T));
+                voff = uint64_t(key) * uint32_t(p.v_token * sizeof(T));
+            }
+            const char* kp = kbase + koff + fetch_byte[i];
+            const char* vp = vbase + voff + fetch_byte[i];
+            if (RD > 32 * NT || !FULL) {  // V's padding: not stored, so any finite or not
+                const bool pad = fetch_byte[i] == ~0u;
+                kp = pad ? reinterpret_cast<const char*>(zero_chunk) : kp;
+                vp = pad ? reinterpret_cast<const char*>(zero_chunk) : vp;
+            }
+            const uint32_t at = stage + (i / PER) * 2 * BLOCK_BYTES + (i % PER) * WAVES * 1024;
+            load_to_lds(kp, at);
+            load_to_lds(vp, at + BLOCK_BYTES);
+        }
+    };
+    load_entries(0);
+
+    // operands: K chunk 2 c + hs of its key's row; f16: V by transpose reads
+    uint32_t koff[DC];
+    const uint32_t krow = kHalf ? perm32(col) : col;
+#pragma unroll
+    for (int c = 0; c < DC; ++c)
+        koff[c] = krow * RD * sizeof(T) + 16 * ((2 * c + hs) ^ lds_swizzle<SW>(krow));
+    constexpr int VOFFS = kHalf ? 2 * NT : 8;
+    uint32_t voff[VOFFS];
+    if constexpr (kHalf) {
+#pragma unroll
+        for (int e2 = 0; e2 < 2; ++e2) {
+            const uint32_t vr = 8 * (lane / 32) + (lane % 16) / 4 + 4 * e2;
+#pragma unroll
+            for (int t = 0; t < NT; ++t) {
+                const uint32_t ch = 2 * ((lane / 16) % 2) + (lane % 4) / 2 + 4 * t;
+                voff[e2 * NT + t] = vr * RD * 2 + 16 * (ch ^ lds_swizzle<SW>(vr)) + 8 * (lane % 2);
+            }
+        }
+    } else {
+        // rows 8 a + 4 hs + b (a < 4, b < 4): their chunk order depends on
+        // (a % 2, b, hs); voff[4 a + b] for a < 2, two rows of eight further for a + 2
+#pragma unroll
+        for (int a = 0; a < 2; ++a)
+#pragma unroll
+            for (int b = 0; b < 4; ++b) {
+                const uint32_t vr = 8 * a + 4 * hs + b;
+                const uint32_t byte = EC * 4 * col;
+                voff[4 * a + b] =
+                    vr * RD * 4 + 16 * ((byte / 16) ^ lds_swizzle<SW>(vr)) + byte % 16;
+            }
+    }
+    typedef typename std::conditional<kHalf, h8, f32x4>::type KV;
+    KV qf[DC];
+    const T* qrow = q + (r.begin + token) * p.q_token + head * p.q_head + CE * hs;
+#pragma unroll
+    for (int c = 0; c < DC; ++c) {
+        const bool in = row_valid && (FULL || uint32_t(2 * CE * c) + CE * hs < hd);
+        qf[c] = in ? *reinterpret_cast<const KV*>(qrow + 2 * CE * c) : KV{};
+    }
+    f32x16 o[NT];
+#pragma unroll
+    for (int t = 0; t < NT; ++t)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) o[t][e] = 0.0f;
+    float m = -INFINITY, l = 0.0f;  // l: this lane's half of the sum
+
+    if (steps > 0) {
+        issue_step(0);
+        load_entries(1);
+    }
+    __builtin_amdgcn_s_waitcnt(0);
+    __syncthreads();
+    for (uint32_t step = 0; step < steps; ++step) {
+        if (step + 1 < steps) {
+            issue_step(step + 1);
+            load_entries(step + 2);
+        }
+        const uint32_t blk = step * KS + share;
+        const uint32_t kbase_key = blk * BN;
+        const unsigned char* ks = lds + (step % 2) * STAGE_BYTES + share * 2 * BLOCK_BYTES;
+        const unsigned char* vs = ks + BLOCK_BYTES;
+        if (blk < blocks && kbase_key < wave_keys) {
+            f32x16 s[KT];
+#pragma unroll
+            for (int kt = 0; kt < KT; ++kt) {
+#pragma unroll
+                for (int e = 0; e < 16; ++e) s[kt][e] = 0.0f;
+#pragma unroll
+                for (int c = 0; c < DC; ++c) {
+                    const KV ka = *reinterpret_cast<const KV*>(
+                        ks + kt * 32 * RD * sizeof(T) + koff[c]);
+                    if constexpr (kHalf) {
+                        s[kt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ka, qf[c], s[kt], 0, 0, 0);
+                    } else {
+#pragma unroll
+                        for (int e = 0; e < 4; ++e)
+                            s[kt] = __builtin_amdgcn_mfma_f32_32x32x2f32(ka[e], qf[c][e], s[kt],
+                                                                         0, 0, 0);
+                    }
+                }
+            }
+            // register e of tile kt: key kbase_key + 32 kt + (f16: 16 (e / 8) + 8 hs + e % 8;
+            // f32: 8 (e / 4) + 4 hs + e % 4)
+            if (kbase_key + BN > wave_least) {
+                const int lim = limit - int(kbase_key) - int((kHalf ? 8 : 4) * hs);
+#pragma unroll
+                for (int kt = 0; kt < KT; ++kt)
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) {
+                        const int at = 32 * kt + (kHalf ? 16 * (e / 8) + e % 8 : 8 * (e / 4) + e % 4);
+                        if (at > lim) s[kt][e] = -INFINITY;
+                    }
+            }
+            float mx = -INFINITY, my = -INFINITY;
+#pragma unroll
+            for (int kt = 0; kt < KT; ++kt)
+#pragma unroll
+                for (int e = 0; e < 16; e += 4) {
+                    mx = max3(mx, s[kt][e], s[kt][e + 1]);
+                    my = max3(my, s[kt][e + 2], s[kt][e + 3]);
+                }
+            mx = halves_max(fmaxf(mx, my)) * p.scale_log2;
+            if (__any(mx > m + kSlack)) {
+                const float m_new = fmaxf(m, mx);
+                const float alpha = m_new > m ? __builtin_amdgcn_exp2f(m - m_new) : 1.0f;
+                m = m_new;
+                l *= alpha;
+#pragma unroll
+                for (int t = 0; t < NT; ++t)
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) o[t][e] *= alpha;
+            }
+            const float neg_m = m == -INFINITY ? 0.0f : -m;
+            if constexpr (kHalf) {
+                // the sum adds the same rounded probabilities that the product takes
+                const h2 ones = {half_t(1.0f), half_t(1.0f)};
+                h8 pb[BN / 16];
+#pragma unroll
+                for (int c = 0; c < BN / 16; ++c) {
+#pragma unroll
+                    for (int e = 0; e < 8; ++e)
+                        pb[c][e] = half_t(__builtin_amdgcn_exp2f(
+                            __builtin_fmaf(s[c / 2][8 * (c % 2) + e], p.scale_log2, neg_m)));
+#pragma unroll
+                    for (int e = 0; e < 8; e += 2)
+                        l = __builtin_amdgcn_fdot2(h2{pb[c][e], pb[c][e + 1]}, ones, l, false);
+                }
+#pragma unroll
+                for (int c = 0; c < BN / 16; ++c)
+#pragma unroll
+                    for (int t = 0; t < NT; ++t) {
+                        const half_t* at = reinterpret_cast<const half_t*>(vs + 16 * c * RD * 2);
+                        const h4 lo = lds_read_transposed(at + voff[t] / 2);
+                        const h4 hi = lds_read_transposed(at + voff[NT + t] / 2);
+                        const h8 va = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+                        o[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(va, pb[c], o[t], 0, 0, 0);
+                    }
+            } else {
+                typedef typename VecOf<float, EC>::type VE;
+#pragma unroll
+                for (int kt = 0; kt < KT; ++kt)
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) {
+                        const float pe = __builtin_amdgcn_exp2f(
+                            __builtin_fmaf(s[kt][e], p.scale_log2, neg_m));
+                        l += pe;
+                        const int a = e / 4, b = e % 4;
+                        const unsigned char* at =
+                            vs + (32 * kt + 16 * (a / 2)) * RD * 4 + voff[4 * (a % 2) + b];
+                        float va[EC];
+                        if constexpr (EC == 3) {  // a row of 96: no 12-byte alignment to chunks
+#pragma unroll
+                            for (int t = 0; t < EC; ++t) {
+                                const uint32_t vr = 32 * kt + 8 * a + 4 * hs + b;
+                                const uint32_t byte = 4 * (EC * col + t);
+                                va[t] = *reinterpret_cast<const float*>(
+                                    vs + vr * RD * 4 + 16 * ((byte / 16) ^ lds_swizzle<SW>(vr)) +
+                                    byte % 16);
+                            }
+                        } else {
+                            const VE w = *reinterpret_cast<const VE*>(at);
+#pragma unroll
+                            for (int t = 0; t < EC; ++t) va[t] = w[t];
+                        }
+#pragma unroll
+                        for (int t = 0; t < NT; ++t)
+                            o[t] = __builtin_amdgcn_mfma_f32_32x32x2f32(va[t], pe, o[t], 0, 0, 0);
+                    }
+            }
+        }
+        __builtin_amdgcn_s_waitcnt(0);  // this wave's share of the next stage has landed
+        __syncthreads();
+    }
+    if (PAGED && __any(bad_page) && lane == 0) any_bad = 1;  // read after the barrier below
+
+    if constexpr (KS > 1) {  // shares 1 .. hand their (max, sum, output) to share 0
+        float* mg = reinterpret_cast<float*>(lds);
+        if (share > 0) {
+            float* dst = mg + ((share - 1) * QW * 64 + qw * 64 + lane) * MERGE;
+            dst[0] = m;
+            dst[1] = l;
+#pragma unroll
+            for (int t = 0; t < NT; ++t)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) dst[2 + 16 * t + e] = o[t][e];
+        }
+        __syncthreads();
+        if (share != 0) return;
+#pragma unroll
+        for (int x = 1; x < KS; ++x) {
+            const float* src = mg + ((x - 1) * QW * 64 + qw * 64 + lane) * MERGE;
+            const float m2 = src[0], top = fmaxf(m, m2);
+            const float a1 = top > m ? __builtin_amdgcn_exp2f(m - top) : 1.0f;
+            const float a2 = top > m2 ? __builtin_amdgcn_exp2f(m2 - top) : 1.0f;
+            l = l * a1 + src[1] * a2;
+#pragma unroll
+            for (int t = 0; t < NT; ++t)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) o[t][e] = o[t][e] * a1 + src[2 + 16 * t + e] * a2;
+            m = top;
+        }
+    } else if (PAGED) {
+        __syncthreads();
+    }
+
+    const float sum = l + __shfl_xor(l, 32, 64);
+    const float inv = limit < 0 ? 0.0f : 1.0f / sum;
+    bool odd = PAGED && any_bad != 0;  // row_by_wave finds which rows see the page
+    if (row_valid) {
+        T* orow = out + (uint64_t(r.begin + token) * p.q_heads + head) * hd;
+#pragma unroll
+        for (int t = 0; t < NT; ++t)
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+                // f16: elements 32 t + 8 g + 4 hs + 0 .. 3; f32: EC (8 g + 4 hs + i) + t
+                typename VecOf<T, 4>::type w;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const float x = limit < 0 ? 0.0f : o[t][4 * g + i] * inv;
+                    const uint32_t d = kHalf ? 32 * t + 8 * g + 4 * hs + i
+                                             : EC * (8 * g + 4 * hs + i) + t;
+                    if (FULL || d < hd) odd |= !(fabsf(x) < INFINITY);
+                    w[i] = r.bad ? T(NAN) : from_float<T>(x);
+                    if (!kHalf && (FULL || d < hd)) orow[d] = w[i];
+                }
+                const uint32_t d = 32 * t + 8 * g + 4 * hs;
+                if (kHalf && (FULL || d < hd))
+                    *reinterpret_cast<typename VecOf<T, 4>::type*>(orow + d) = w;
+            }
+    }
+    if (r.bad) return;
+    // rows with an output that is not finite once more, by the whole wave (after
+    // its own stores above)
+    const uint64_t votes = __ballot(odd && row_valid);
+    uint32_t redo = uint32_t(votes | votes >> 32);
+    if (redo == 0) return;
+    __builtin_amdgcn_s_waitcnt(0);
+    for (; redo != 0; redo &= redo - 1) {
+        const uint32_t again = wrow0 + __builtin_ctz(redo);
+        row_by_wave<T, PAGED>(q, k, v, out, p, request, r, again / p.group,
+                              kvh * p.group + again % p.group);
+    }
+}
+
 // -------------------------------------------------------------- workspace
 //
 // The split kernel's partials and tickets.  Its workgroups a KV head: `share`
@@ -763,6 +1227,41 @@ void launch_rows(rl_context* ctx, const T* q, const T* k, const T* v, T* out,
         RL_LAUNCH(ctx, (k_ragged_rows<T, 8, PAGED>), grid, block, q, k, v, out, p);
 }
 
+// The tile kernel for a batch of at most `tokens` rows.
+template <typename T, int NT, int QW, int KS, int BN, bool PAGED>
+void launch_tiles(rl_context* ctx, const T* q, const T* k, const T* v, T* out,
+                  const RaggedParams& p) {
+    const uint64_t units =
+        uint64_t(p.tokens) * p.group / kTileRows<QW> + p.sequences;
+    const dim3 grid(uint32_t(units * p.kv_heads)), block(64 * QW * KS);
+    if (p.head_dim == 32 * NT)
+        RL_LAUNCH(ctx, (k_ragged_tiles<T, NT, QW, KS, BN, PAGED, true>), grid, block, q, k, v, out,
+                  p);
+    else
+        RL_LAUNCH(ctx, (k_ragged_tiles<T, NT, QW, KS, BN, PAGED, false>), grid, block, q, k, v,
+                  out, p);
+}
+template <typename T, bool PAGED>
+void launch_tiles(rl_context* ctx, const T* q, const T* k, const T* v, T* out,
+                  const RaggedParams& p) {
+    constexpr bool kHalf = std::is_same<T, half_t>::value;
+    const uint64_t wide =
+        (uint64_t(p.tokens) * p.group / kTileRows<4>) * p.kv_heads;
+    const uint32_t nt = (p.head_dim + 31) / 32;
+    constexpr int B64 = kHalf ? 64 : 32;  // keys of a block: 8 KB of K for 64 elements a row
+    if (wide >= uint64_t(ctx->num_cus)) {
+        if (nt == 1) launch_tiles<T, 1, 4, 1, B64, PAGED>(ctx, q, k, v, out, p);
+        else if (nt == 2) launch_tiles<T, 2, 4, 1, B64, PAGED>(ctx, q, k, v, out, p);
+        else if (nt == 3) launch_tiles<T, 3, 4, 1, B64, PAGED>(ctx, q, k, v, out, p);
+        else launch_tiles<T, 4, 4, 1, B64, PAGED>(ctx, q, k, v, out, p);
+    } else {
+        if (nt == 1) launch_tiles<T, 1, 1, 4, B64, PAGED>(ctx, q, k, v, out, p);
+        else if (nt == 2) launch_tiles<T, 2, 1, 4, 32, PAGED>(ctx, q, k, v, out, p);
+        else if (nt == 3) launch_tiles<T, 3, 1, 2, 32, PAGED>(ctx, q, k, v, out, p);
+        else launch_tiles<T, 4, 1, 2, 32, PAGED>(ctx, q, k, v, out, p);
+    }
+}
+
 template <typename T>
 void launch_split(rl_context* ctx, const T* q, const T* k, const T* v, T* out,
                   const RaggedParams& p) {
@@ -817,8 +1316,21 @@ rl_status packed_entry(rl_context* ctx, const char* name, const rl_buffer* q,
     p.v_head = v_strides[1];
     p.scale = scale;
     p.scale_log2 = scale * kLog2e;
-    launch_rows<T, false>(ctx, static_cast<const T*>(q->data), static_cast<const T*>(k->data),
-                          static_cast<const T*>(v->data), static_cast<T*>(out->data), p);
+    const T* qd = static_cast<const T*>(q->data);
+    const T* kd = static_cast<const T*>(k->data);
+    const T* vd = static_cast<const T*>(v->data);
+    T* od = static_cast<T*>(out->data);
+    // the matrix-core kernel: rows of whole 16-byte pieces on their grid, up to
+    // 128 elements, row strides that fit its 32-bit byte steps
+    bool matrix = D * es % 16 == 0 && D <= 128 && aligned_to(qd, 16) && aligned_to(kd, 16) &&
+                  aligned_to(vd, 16) && aligned_to(od, 16);
+    for (const uint64_t* strides : {q_strides, k_strides, v_strides})
+        matrix = matrix && strides[0] * es % 16 == 0 && strides[1] * es % 16 == 0 &&
+                 strides[0] <= UINT32_MAX / es;
+    if (matrix)
+        launch_tiles<T, false>(ctx, qd, kd, vd, od, p);
+    else
+        launch_rows<T, false>(ctx, qd, kd, vd, od, p);
     return after_launch(ctx, name);
 }
 
@@ -904,22 +1416,25 @@ rl_status paged_entry(rl_context* ctx, const char* name, const rl_buffer* q,
     const uint64_t page_bytes = kv_heads * page_size * head_dim * es;
     const bool matrix = head_dim * es % 16 == 0 && head_dim <= 128 && page_size >= 8 &&
                         page_bytes <= UINT32_MAX && aligned_to(qd, 16) && aligned_to(kd, 16) &&
-                        aligned_to(vd, 16);
+                        aligned_to(vd, 16) && aligned_to(od, 16);
     const uint64_t most_rows = std::min(max_queries, tokens) * p.group;
+    p.page_bytes = uint32_t(page_bytes);
+    p.head_bytes = uint32_t(page_size * head_dim * es);
     if (matrix && p.group <= kSplitRows) {
         char* ws = static_cast<char*>(workspace->data);
         p.small_rows = kSplitRows;
         p.share = uint32_t(w.share);
         p.splits = uint32_t(w.splits);
-        p.page_bytes = uint32_t(page_bytes);
-        p.head_bytes = uint32_t(page_size * head_dim * es);
         p.tickets = reinterpret_cast<uint32_t*>(ws);
         p.part = reinterpret_cast<float*>(ws + held->second.ticket_bytes);
         p.part_ml = p.part + w.splits * kv_heads * kSplitRows * 128;
         launch_split<T>(ctx, qd, kd, vd, od, p);
         if (most_rows <= kSplitRows) return after_launch(ctx, name);
     }
-    launch_rows<T, true>(ctx, qd, kd, vd, od, p);
+    if (matrix)
+        launch_tiles<T, true>(ctx, qd, kd, vd, od, p);
+    else
+        launch_rows<T, true>(ctx, qd, kd, vd, od, p);
     return after_launch(ctx, name);
 }
 
