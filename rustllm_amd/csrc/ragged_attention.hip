@@ -52,12 +52,11 @@ struct RaggedParams {
     // to the split kernel: it takes those, the others skip them.
     uint32_t small_rows;
     // split kernel
-    uint32_t splits;       // workgroups a KV head has for its requests' key ranges
-    uint32_t share;        // key units a KV head's workgroups are sized for
+    uint32_t slots;        // workgroups a KV head can have running at once
     uint32_t page_bytes;   // of one page, all KV heads
     uint32_t head_bytes;   // of one KV head's rows in a page
-    float* part;           // [workgroup][16][head size]: unnormalised outputs
-    float* part_ml;        // [workgroup][16]: (max in log2 units, sum)
+    float* part;           // [workgroup][2][16][head size, padded]: unnormalised outputs
+    float* part_ml;        // [workgroup][2][16]: (max in log2 units, sum)
     uint32_t* tickets;     // [request][KV head], kTicketStride words apart
 };
 
@@ -267,24 +266,24 @@ __global__ __launch_bounds__(64) void k_ragged_rows(const T* __restrict__ q,
 // V^T P^T, per wave in its own registers.
 //
 // Work: every request's keys are cut into units of 4 kKeys (one block of kKeys
-// for each of a workgroup's four waves), and the units of all requests into
-// ranges of the same count, one a workgroup, no range over two requests.  The
-// lengths are only here, so every workgroup finds its range itself: a wave sums
-// the units over the requests, which gives the count per range, and a second
-// sum gives its request.  Partials of a request in several ranges meet by a
-// ticket: the workgroup that finishes last merges them.
+// for each of a workgroup's four waves), and all units, request after request,
+// dealt out in equal shares to as many workgroups as run at once (two a CU).
+// The lengths are only here, so every workgroup finds its share itself, by a
+// sum over the requests.  Requests that lie in several shares leave partials,
+// which meet by a ticket: the workgroup that finishes last merges them.
 //
 // Layout: K's operand is its rows as they lie in memory (16 bytes a lane).  V's
 // has to come by columns: a lane loads its 4 or 8 columns of eight
 // neighbouring rows (f32: of four) and takes the operand of each column across
 // those registers (v_perm), so nothing passes through LDS.  Rows of the score
 // tiles are keys in the order that leaves a lane the probabilities of exactly
-// those eight rows.  The next block's K and V are in flight while one is
-// computed, and the page entries one block further ahead.  Bound by HBM.
+// those eight rows.  A block's registers are refilled as soon as its scores (K)
+// and products (V) are through, so the next block's rows are in flight under
+// the rest of the work; its page entries are read a block ahead.  Bound by HBM.
 template <typename T, int DP>
 struct SplitShape {
     static constexpr bool kHalf = std::is_same<T, half_t>::value;
-    static constexpr int kKeys = (kHalf ? 4096 : 2048) / DP;  // keys of a block
+    static constexpr int kKeys = kHalf ? 32 : 16;             // keys of a block
     static constexpr int kKTiles = kKeys / 16;
     static constexpr int kKChunks = kHalf ? DP / 32 : DP / 16;  // 16-byte pieces of a K row a lane
     static constexpr int kVRows = kHalf ? 8 : 4;                // neighbouring V rows a lane
@@ -335,10 +334,10 @@ __device__ inline float2 observe2(const float* p) {
 }
 
 // A request's units for the split kernel, 0 if it is not one of its own.
-__device__ inline uint32_t split_units(const RaggedParams& p, uint32_t i, uint32_t unit_shift) {
-    if (i >= p.sequences) return 0u;
-    const Request r = load_request<true>(p, i);
-    if (r.n == 0 || r.n * p.group > p.small_rows) return 0u;
+__device__ inline uint32_t split_units(const RaggedParams& p, uint32_t i, uint32_t unit_shift,
+                                       Request& r) {
+    r = load_request<true>(p, min(i, p.sequences - 1));
+    if (i >= p.sequences || r.n == 0 || r.n * p.group > p.small_rows) return 0u;
     // no keys to read where every row is zero or NaN: one unit writes them
     const uint32_t units = uint32_t((uint64_t(r.keys) + (1u << unit_shift) - 1) >> unit_shift);
     return r.bad || units == 0 ? 1u : units;
@@ -379,37 +378,54 @@ __global__ __launch_bounds__(64 * kSplitWaves, 2) void k_ragged_split(
     const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
     const uint32_t lane = threadIdx.x % 64;
     const uint32_t lr = lane % 16, g = lane / 16;
-    const uint32_t kvh = blockIdx.x % p.kv_heads, w = blockIdx.x / p.kv_heads;
+    const uint32_t kvh = blockIdx.x % p.kv_heads;
+    const uint64_t w = blockIdx.x / p.kv_heads;
 
-    // this workgroup's request and key range
-    const uint32_t units0 = split_units(p, lane, kUnitShift);  // of the first 64 requests
-    uint64_t total = last_lane(wave_scan(units0));
+    // Every workgroup's share of the units: `per` of them in request order.
+    Request lane0;  // of the first 64 requests
+    const uint32_t units0 = split_units(p, lane, kUnitShift, lane0);
+    const uint32_t upto0 = wave_scan(units0);
+    uint64_t total = last_lane(upto0);
+    Request other;
     for (uint32_t base = 64; base < p.sequences; base += 64)
-        total += last_lane(wave_scan(split_units(p, base + lane, kUnitShift)));
-    const uint32_t per = max(1u, uint32_t((total + p.share - 1) / p.share));
-    uint32_t before = 0, request = p.sequences, first_split = 0, n_splits = 0;
+        total += last_lane(wave_scan(split_units(p, base + lane, kUnitShift, other)));
+    const uint64_t per = max(uint64_t(1), (total + p.slots - 1) / p.slots);
+    const uint64_t end = min(total, (w + 1) * per);
+    for (uint64_t at = w * per; at < end;) {
+    // the request of unit `at`: the first whose units end past it
+    uint32_t request = 0, units = 0;
+    uint64_t first = 0;  // its first unit
+    Request r{};
     for (uint32_t base = 0; base < p.sequences; base += 64) {
-        const uint32_t units = base == 0 ? units0 : split_units(p, base + lane, kUnitShift);
-        const uint32_t mine = (units + per - 1) / per;
-        const uint32_t upto = before + wave_scan(mine);
-        const uint64_t past = __ballot(upto > w);
+        other = lane0;
+        const uint32_t mine =
+            base == 0 ? units0 : split_units(p, base + lane, kUnitShift, other);
+        const uint32_t upto = base == 0 ? upto0 : wave_scan(mine);
+        const uint64_t past = __ballot(first + upto > at);
         if (past != 0) {
-            const int at = __builtin_ctzll(past);
-            request = base + at;
-            n_splits = uint32_t(__builtin_amdgcn_readlane(int(mine), at));
-            first_split = uint32_t(__builtin_amdgcn_readlane(int(upto), at)) - n_splits;
+            const int in = __builtin_ctzll(past);
+            request = base + in;
+            units = uint32_t(__builtin_amdgcn_readlane(int(mine), in));
+            first += uint32_t(__builtin_amdgcn_readlane(int(upto), in)) - units;
+            r.begin = uint32_t(__builtin_amdgcn_readlane(int(other.begin), in));
+            r.n = uint32_t(__builtin_amdgcn_readlane(int(other.n), in));
+            r.keys = uint32_t(__builtin_amdgcn_readlane(int(other.keys), in));
+            r.bad = __builtin_amdgcn_readlane(int(other.bad), in) != 0;
+            r.first = int64_t(r.keys) - r.n;
             break;
         }
-        before = last_lane(upto);
+        first += last_lane(upto);
     }
-    if (request >= p.sequences) return;  // more workgroups than ranges
-    const Request r = load_request<true>(p, request);
-    const uint32_t split = w - first_split;
+    const uint64_t w0 = first / per;  // workgroups w0 .. w0 + n_splits - 1 share the request
+    const uint32_t n_splits = uint32_t((first + units - 1) / per - w0) + 1;
+    const uint32_t split = uint32_t(w - w0);
+    const uint32_t u0 = uint32_t(at - first), u1 = uint32_t(min(uint64_t(units), end - first));
+    at = first + u1;
     const uint32_t R = r.n * p.group;
     const uint32_t last = r.keys == 0 ? 0u : r.keys - 1;
     const uint32_t blocks = r.bad ? 0u : (r.keys + kKeys - 1) / kKeys;
-    const uint32_t b0 = split * per * kSplitWaves;
-    const uint32_t b1 = min(blocks, b0 + per * kSplitWaves);
+    const uint32_t b0 = u0 * kSplitWaves;
+    const uint32_t b1 = min(blocks, u1 * kSplitWaves);
 
     const uint32_t* entries = p.table + uint64_t(request) * p.max_blocks;
     bool bad_page = false;
@@ -427,7 +443,8 @@ __global__ __launch_bounds__(64 * kSplitWaves, 2) void k_ragged_split(
     // columns kVCols lr .. of V, those past the head size read the first ones
     const uint32_t col = S::kVCols * lr;
     const char* vbase = reinterpret_cast<const char*>(v) + uint64_t(kvh) * p.head_bytes;
-    auto load_block = [&](Block& x, uint32_t blk, uint32_t entry) {
+    Block x;
+    auto load_keys = [&](uint32_t blk, uint32_t entry) {
         const uint32_t kb = blk * kKeys;
 #pragma unroll
         for (int m = 0; m < S::kKTiles; ++m) {
@@ -442,6 +459,9 @@ __global__ __launch_bounds__(64 * kSplitWaves, 2) void k_ragged_split(
                 x.k[m][c] = in ? *reinterpret_cast<const KV*>(row + 64 * c) : KV{};
             }
         }
+    };
+    auto load_values = [&](uint32_t blk, uint32_t entry) {
+        const uint32_t kb = blk * kKeys;
 #pragma unroll
         for (int t = 0; t < S::kVSteps; ++t) {
             const uint32_t run = kb + 4 * S::kVRows * t + S::kVRows * g;  // inside one page
@@ -480,8 +500,8 @@ __global__ __launch_bounds__(64 * kSplitWaves, 2) void k_ragged_split(
     for (int t = 0; t < S::kTiles; ++t) o[t] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
     float m = -INFINITY, l = 0.0f;  // l: this lane's share
 
-    auto compute = [&](const Block& x, uint32_t blk) {
-        f32x4 s[S::kKTiles];
+    f32x4 s[S::kKTiles];
+    auto scores = [&] {
 #pragma unroll
         for (int t = 0; t < S::kKTiles; ++t) {
             s[t] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
@@ -497,6 +517,8 @@ __global__ __launch_bounds__(64 * kSplitWaves, 2) void k_ragged_split(
                 }
             }
         }
+    };
+    auto weights = [&](uint32_t blk) {
         // register r of tile t: key blk kKeys + (a constant) + 8 g (f32: 4 g)
         const int seen = limit - int(blk * kKeys) - int(S::kVRows * g);
         float mx = -INFINITY;
@@ -523,6 +545,8 @@ __global__ __launch_bounds__(64 * kSplitWaves, 2) void k_ragged_split(
 #pragma unroll
             for (int e = 0; e < 4; ++e)
                 s[t][e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[t][e], p.scale_log2, -shift));
+    };
+    auto values = [&] {
         if constexpr (kHalf) {
 #pragma unroll
             for (int t = 0; t < S::kVSteps; ++t) {
@@ -556,36 +580,29 @@ __global__ __launch_bounds__(64 * kSplitWaves, 2) void k_ragged_split(
 
     uint32_t blk = b0 + wave;
     if (blk < b1) {
-        Block a, b;
-        uint32_t entry = load_entry(blk);
+        uint32_t entry = checked(load_entry(blk));
+        load_keys(blk, entry);
+        load_values(blk, entry);
         uint32_t ahead = load_entry(min(blk + kSplitWaves, b1 - 1));
-        load_block(a, blk, checked(entry));
-        while (true) {
-            if (blk + kSplitWaves >= b1) {
-                compute(a, blk);
-                break;
-            }
-            entry = ahead;
+        for (; blk + kSplitWaves < b1; blk += kSplitWaves) {
+            scores();
+            entry = checked(ahead);
             ahead = load_entry(min(blk + 2 * kSplitWaves, b1 - 1));
-            load_block(b, blk + kSplitWaves, checked(entry));
-            compute(a, blk);
-            blk += kSplitWaves;
-            if (blk + kSplitWaves >= b1) {
-                compute(b, blk);
-                break;
-            }
-            entry = ahead;
-            ahead = load_entry(min(blk + 2 * kSplitWaves, b1 - 1));
-            load_block(a, blk + kSplitWaves, checked(entry));
-            compute(b, blk);
-            blk += kSplitWaves;
+            load_keys(blk + kSplitWaves, entry);
+            weights(blk);
+            values();
+            load_values(blk + kSplitWaves, entry);
         }
+        scores();
+        weights(blk);
+        values();
     }
     l = columns_sum(l);
     if (__any(bad_page)) l = NAN;  // row_by_wave finds which rows see it
 
     // the four waves' states -> the range's.  Lane (g, lr), f16: elements
     // kTiles (4 g + e) + c of row lr in o[c][e]; f32: 64 (c / 4) + 4 (4 g + e) + c % 4.
+    __syncthreads();  // the share's previous request is through with the LDS
     if (threadIdx.x == 0) odd_rows = 0;
     if (g == 0) {
         merge_ml[wave][lr][0] = m;
@@ -600,7 +617,10 @@ __global__ __launch_bounds__(64 * kSplitWaves, 2) void k_ragged_split(
             merge_o[wave][lr][at] = o[c][e];
         }
     __syncthreads();
-    const uint32_t slot = kvh * p.splits + w;
+    // partials: a workgroup can hold one of a request that began before its share
+    // and one of a request that goes on behind it
+    const uint64_t slot0 = (uint64_t(kvh) * p.slots + w0) * 2;
+    const uint64_t slot = slot0 + 2 * split + (split == 0);
     const uint32_t pairs = hd / 2;
     // row `row`'s output, two elements: stored unless it is not finite
     auto store_row = [&](uint32_t row, uint32_t d, float2 x, float sum) {
@@ -633,8 +653,8 @@ __global__ __launch_bounds__(64 * kSplitWaves, 2) void k_ragged_split(
         if (n_splits == 1) {
             store_row(row, d, acc, sum);
         } else {
-            publish2(p.part + (uint64_t(slot) * kSplitRows + row) * DP + d, acc.x, acc.y);
-            if (d == 0) publish2(p.part_ml + (uint64_t(slot) * kSplitRows + row) * 2, top, sum);
+            publish2(p.part + (slot * kSplitRows + row) * DP + d, acc.x, acc.y);
+            if (d == 0) publish2(p.part_ml + (slot * kSplitRows + row) * 2, top, sum);
         }
     }
     if (n_splits > 1) {
@@ -652,12 +672,11 @@ __global__ __launch_bounds__(64 * kSplitWaves, 2) void k_ragged_split(
             ticket = __hip_atomic_fetch_add(counter, 1u, __ATOMIC_RELAXED,
                                             __HIP_MEMORY_SCOPE_AGENT);
         __syncthreads();
-        if (ticket != n_splits - 1) return;
+        if (ticket != n_splits - 1) continue;
         __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "agent");
         if (threadIdx.x == 0)  // for the next call
             __hip_atomic_store(counter, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
         constexpr uint32_t kChunk = 8;
-        const uint64_t slot0 = uint64_t(kvh) * p.splits + first_split;
         for (uint32_t i = threadIdx.x; i < R * pairs; i += 64 * kSplitWaves) {
             const uint32_t row = i / pairs, d = 2 * (i % pairs);
             float top = -INFINITY, sum = 0.0f;
@@ -666,10 +685,10 @@ __global__ __launch_bounds__(64 * kSplitWaves, 2) void k_ragged_split(
                 float2 ml[kChunk], ov[kChunk];
 #pragma unroll
                 for (uint32_t x = 0; x < kChunk; ++x) {
-                    const uint64_t at =
-                        (slot0 + min(s0 + x, n_splits - 1)) * kSplitRows + row;
-                    ml[x] = observe2(p.part_ml + at * 2);
-                    ov[x] = observe2(p.part + at * DP + d);
+                    const uint32_t n = min(s0 + x, n_splits - 1);
+                    const uint64_t from = (slot0 + 2 * n + (n == 0)) * kSplitRows + row;
+                    ml[x] = observe2(p.part_ml + from * 2);
+                    ov[x] = observe2(p.part + from * DP + d);
                 }
                 float next = top;
 #pragma unroll
@@ -703,6 +722,7 @@ __global__ __launch_bounds__(64 * kSplitWaves, 2) void k_ragged_split(
         row_by_wave<T, true>(q, k, v, out, p, request, r, row / p.group,
                              kvh * p.group + row % p.group);
     }
+    }  // the next request of this workgroup's share
 }
 
 // -------------------------------------------------- many rows per KV head
@@ -1171,23 +1191,18 @@ __global__ __launch_bounds__(64 * QW * KS, (kTileWaves<T, NT, QW, KS, BN>)) void
 
 // -------------------------------------------------------------- workspace
 //
-// The split kernel's partials and tickets.  Its workgroups a KV head: `share`
-// equal ranges of all units, and up to one more a request for the ranges that
-// end with it.  Ranges are counted for two workgroups a CU, its registers'
-// occupancy; several requests of different lengths leave short last ranges, so
-// they are cut finer.
+// The split kernel's workgroups (two fit a CU: registers), their partials and
+// tickets.
 struct WorkspaceNeed {
-    uint64_t share, splits;
+    uint64_t slots;
     rl_context::Workspace size;
 };
 
 WorkspaceNeed workspace_for(const rl_context* ctx, uint64_t sequences, uint64_t kv_heads) {
     WorkspaceNeed w{};
-    const uint64_t rounds = sequences == 1 ? 1 : sequences < 4 ? 2 : 4;
-    w.share = ceil_div(rounds * 2 * uint64_t(ctx->num_cus), kv_heads);
-    w.splits = w.share + sequences;
+    w.slots = std::max<uint64_t>(2 * uint64_t(ctx->num_cus) / kv_heads, 1);
     w.size.ticket_bytes = sequences * kv_heads * kTicketStride * sizeof(uint32_t);
-    w.size.partial_bytes = w.splits * kv_heads * kSplitRows * (128 + 2) * sizeof(float);
+    w.size.partial_bytes = 2 * w.slots * kv_heads * kSplitRows * (128 + 2) * sizeof(float);
     return w;
 }
 
@@ -1265,7 +1280,7 @@ void launch_tiles(rl_context* ctx, const T* q, const T* k, const T* v, T* out,
 template <typename T>
 void launch_split(rl_context* ctx, const T* q, const T* k, const T* v, T* out,
                   const RaggedParams& p) {
-    const dim3 grid(p.splits * p.kv_heads), block(64 * kSplitWaves);
+    const dim3 grid(p.slots * p.kv_heads), block(64 * kSplitWaves);
     if (p.head_dim == 64)
         RL_LAUNCH(ctx, (k_ragged_split<T, 64, true>), grid, block, q, k, v, out, p);
     else if (p.head_dim < 64)
@@ -1423,11 +1438,10 @@ rl_status paged_entry(rl_context* ctx, const char* name, const rl_buffer* q,
     if (matrix && p.group <= kSplitRows) {
         char* ws = static_cast<char*>(workspace->data);
         p.small_rows = kSplitRows;
-        p.share = uint32_t(w.share);
-        p.splits = uint32_t(w.splits);
+        p.slots = uint32_t(w.slots);
         p.tickets = reinterpret_cast<uint32_t*>(ws);
         p.part = reinterpret_cast<float*>(ws + held->second.ticket_bytes);
-        p.part_ml = p.part + w.splits * kv_heads * kSplitRows * 128;
+        p.part_ml = p.part + 2 * w.slots * kv_heads * kSplitRows * 128;
         launch_split<T>(ctx, qd, kd, vd, od, p);
         if (most_rows <= kSplitRows) return after_launch(ctx, name);
     }
