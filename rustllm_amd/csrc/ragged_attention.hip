@@ -51,6 +51,7 @@ struct RaggedParams {
     // Requests of at most this many rows a KV head (tokens times group) belong
     // to the split kernel: it takes those, the others skip them.
     uint32_t small_rows;
+    bool longest_first;  // tile kernel: order of the tiles
     // split kernel
     uint32_t slots;        // workgroups a KV head can have running at once
     uint32_t page_bytes;   // of one page, all KV heads
@@ -813,7 +814,45 @@ __device__ inline uint32_t find_tile_request(const RaggedParams& p, uint32_t u, 
 // four waves fit a CU's LDS.
 template <typename T, int NT, int QW, int KS, int BN>
 constexpr int kTileWaves =
-    QW * KS == 4 && 2 * KS * 2 * BN * (NT == 3 ? 128 : 32 * NT) * int(sizeof(T)) <= 72 * 1024 ? 2 : 1;
+    QW * KS == 4 && BN == 32 && NT == 4 ? 3 : QW * KS == 4 && 2 * KS * 2 * BN * (NT == 3 ? 128 : 32 * NT) * int(sizeof(T)) <= 72 * 1024 ? 2 : 1;
+
+// Up to 64 requests: tile u in the order of the keys that tiles see, most
+// first (in steps of a tile's tokens), so that the long ones do not start last.
+// Lane i counts request i's tiles at or past a level; the tile's level is the
+// largest that u + 1 tiles reach.  Returns the request, its tile in `tile`;
+// `sequences` if there are not that many tiles.
+template <bool PAGED>
+__device__ inline uint32_t find_longest_tile(const RaggedParams& p, uint32_t u, uint32_t rows,
+                                             uint32_t& tile) {
+    const uint32_t lane = threadIdx.x % 64;
+    const Request r = load_request<PAGED>(p, min(lane, p.sequences - 1));
+    const bool mine = lane < p.sequences && r.n * p.group > p.small_rows;
+    const uint32_t tiles = mine ? (r.n * p.group + rows - 1) / rows : 0u;
+    const uint32_t low = r.first <= 0 ? 0u : uint32_t(uint64_t(r.first) * p.group / rows);
+    auto reach = [&](uint32_t level) {  // this request's tiles at or past it
+        return min(tiles, low + tiles > level ? low + tiles - level : 0u);
+    };
+    uint32_t lo = 0, hi = 1;  // N(lo) > u >= N(hi) once hi is past all levels
+    if (last_lane(wave_scan(tiles)) <= u) return p.sequences;
+    while (last_lane(wave_scan(reach(hi))) > u) {
+        lo = hi;
+        hi *= 2;
+    }
+    while (hi - lo > 1) {
+        const uint32_t mid = lo + (hi - lo) / 2;
+        if (last_lane(wave_scan(reach(mid))) > u) lo = mid;
+        else hi = mid;
+    }
+    const uint32_t before = last_lane(wave_scan(reach(lo + 1)));
+    const uint32_t upto = wave_scan(reach(lo) - reach(lo + 1));
+    const int at = __builtin_ctzll(__ballot(upto > u - before));
+    // the level's tile of that request: all of its lower ones where it starts past the level
+    tile = uint32_t(__builtin_amdgcn_readlane(int(tiles), at)) -
+           uint32_t(__builtin_amdgcn_readlane(int(reach(lo)), at)) +
+           (u - before - (uint32_t(__builtin_amdgcn_readlane(int(upto), at)) -
+                          uint32_t(__builtin_amdgcn_readlane(int(reach(lo) - reach(lo + 1)), at))));
+    return uint32_t(at);
+}
 
 template <typename T, int NT, int QW, int KS, int BN, bool PAGED, bool FULL>
 __global__ __launch_bounds__(64 * QW * KS, (kTileWaves<T, NT, QW, KS, BN>)) void k_ragged_tiles(
@@ -838,20 +877,28 @@ __global__ __launch_bounds__(64 * QW * KS, (kTileWaves<T, NT, QW, KS, BN>)) void
     constexpr int MERGE = NT * 16 + 2;
     constexpr int MERGE_BYTES = (KS - 1) * QW * 64 * MERGE * 4;
     constexpr int LDS_BYTES = 2 * STAGE_BYTES > MERGE_BYTES ? 2 * STAGE_BYTES : MERGE_BYTES;
-    static_assert(BLOCK_CHUNKS % (64 * WAVES) == 0, "a wave's loads cover whole blocks");
+    static_assert(BLOCK_CHUNKS % 64 == 0 && BLOCK_CHUNKS * KS % THREADS == 0,
+                  "a wave's load stays in one block");
     __shared__ __align__(16) unsigned char lds[LDS_BYTES];
     __shared__ uint32_t any_bad;
 
     const uint32_t hd = FULL ? uint32_t(D) : p.head_dim;
     const uint32_t kvh = blockIdx.x % p.kv_heads;
-    const uint32_t units = gridDim.x / p.kv_heads;
-    const uint32_t unit = units - 1 - blockIdx.x / p.kv_heads;
-    const uint32_t request = find_tile_request(p, unit, TILE);
-    const uint32_t tile0 = tiles_before(p, request, TILE);
+    const uint32_t unit = blockIdx.x / p.kv_heads;
+    uint32_t request, tile;
+    if (p.longest_first) {
+        request = find_longest_tile<PAGED>(p, unit, TILE, tile);
+        if (request >= p.sequences) return;
+    } else {
+        const uint32_t back = gridDim.x / p.kv_heads - 1 - unit;
+        request = find_tile_request(p, back, TILE);
+        tile = back - tiles_before(p, request, TILE);
+        if (back < tiles_before(p, request, TILE)) return;
+    }
     const Request r = load_request<PAGED>(p, request);
     const uint32_t rows = r.n * p.group;
-    const uint32_t row0 = (unit - tile0) * TILE;
-    if (unit < tile0 || row0 >= rows || rows <= p.small_rows) return;
+    if (uint64_t(tile) * TILE >= rows || rows <= p.small_rows) return;
+    const uint32_t row0 = tile * TILE;
 
     const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
     const uint32_t lane = threadIdx.x % 64;
@@ -882,12 +929,11 @@ __global__ __launch_bounds__(64 * QW * KS, (kTileWaves<T, NT, QW, KS, BN>)) void
     uint32_t fetch_byte[LOADS];  // of the chunk in its row; ~0u: padding
 #pragma unroll
     for (int i = 0; i < LOADS; ++i) {
-        // instruction i of a wave fills 64 chunks in a row of share i / PER's block
-        constexpr int PER = BLOCK_CHUNKS / (64 * WAVES);
-        const uint32_t c = ((i % PER) * WAVES + wave) * 64 + lane;  // chunk in the block
+        // load i of a wave fills 64 chunks in a row, of one share's block
+        const uint32_t all = (i * WAVES + wave) * 64 + lane, c = all % BLOCK_CHUNKS;
         const uint32_t kr = c / ROW_CHUNKS;
         const uint32_t ch = (c % ROW_CHUNKS) ^ lds_swizzle<SW>(kr);
-        fetch_key[i] = (i / PER) * BN + kr;
+        fetch_key[i] = (all / BLOCK_CHUNKS) * BN + kr;
         fetch_byte[i] = ch * CE < hd ? 16 * ch : ~0u;
     }
     const uint32_t lds_base = uint32_t(
@@ -913,12 +959,12 @@ __global__ __launch_bounds__(64 * QW * KS, (kTileWaves<T, NT, QW, KS, BN>)) void
         }
     };
     auto issue_step = [&](uint32_t step) {
-        const uint32_t stage = __builtin_amdgcn_readfirstlane(
-            lds_base + (step % 2) * STAGE_BYTES + 16 * 64 * wave);
+        const uint32_t stage =
+            __builtin_amdgcn_readfirstlane(lds_base + (step % 2) * STAGE_BYTES);
 #pragma unroll
         for (int i = 0; i < LOADS; ++i) {
-            constexpr int PER = BLOCK_CHUNKS / (64 * WAVES);
-            if (step * KS + i / PER >= blocks) continue;
+            const uint32_t first = (i * WAVES + wave) * 64;  // chunk, over the shares' blocks
+            if (step * KS + first / BLOCK_CHUNKS >= blocks) continue;
             const uint32_t key = min(step * KS * BN + fetch_key[i], last);
             uint64_t koff, voff;
             if constexpr (PAGED) {
@@ -938,7 +984,7 @@ __global__ __launch_bounds__(64 * QW * KS, (kTileWaves<T, NT, QW, KS, BN>)) void
                 kp = pad ? reinterpret_cast<const char*>(zero_chunk) : kp;
                 vp = pad ? reinterpret_cast<const char*>(zero_chunk) : vp;
             }
-            const uint32_t at = stage + (i / PER) * 2 * BLOCK_BYTES + (i % PER) * WAVES * 1024;
+            const uint32_t at = stage + 16 * first + first / BLOCK_CHUNKS * BLOCK_BYTES;
             load_to_lds(kp, at);
             load_to_lds(vp, at + BLOCK_BYTES);
         }
@@ -1242,6 +1288,8 @@ void launch_rows(rl_context* ctx, const T* q, const T* k, const T* v, T* out,
         RL_LAUNCH(ctx, (k_ragged_rows<T, 8, PAGED>), grid, block, q, k, v, out, p);
 }
 
+constexpr uint64_t kManyTiles = 1;
+constexpr uint64_t kSomeTiles = 1000000;
 // The tile kernel for a batch of at most `tokens` rows.
 template <typename T, int NT, int QW, int KS, int BN, bool PAGED>
 void launch_tiles(rl_context* ctx, const T* q, const T* k, const T* v, T* out,
@@ -1257,18 +1305,26 @@ void launch_tiles(rl_context* ctx, const T* q, const T* k, const T* v, T* out,
                   out, p);
 }
 template <typename T, bool PAGED>
-void launch_tiles(rl_context* ctx, const T* q, const T* k, const T* v, T* out,
-                  const RaggedParams& p) {
+void launch_tiles(rl_context* ctx, const T* q, const T* k, const T* v, T* out, RaggedParams p) {
     constexpr bool kHalf = std::is_same<T, half_t>::value;
     const uint64_t wide =
         (uint64_t(p.tokens) * p.group / kTileRows<4>) * p.kv_heads;
     const uint32_t nt = (p.head_dim + 31) / 32;
+    const uint64_t slots = (nt <= 2 ? 4 : 2) * uint64_t(ctx->num_cus);  // wide tiles at once
+    p.longest_first = p.sequences <= 64 && wide >= slots && wide <= 3 * slots;
     constexpr int B64 = kHalf ? 64 : 32;  // keys of a block: 8 KB of K for 64 elements a row
-    if (wide >= uint64_t(ctx->num_cus)) {
+    if (wide >= kManyTiles * uint64_t(ctx->num_cus)) {
         if (nt == 1) launch_tiles<T, 1, 4, 1, B64, PAGED>(ctx, q, k, v, out, p);
-        else if (nt == 2) launch_tiles<T, 2, 4, 1, B64, PAGED>(ctx, q, k, v, out, p);
+        else if (nt == 2) launch_tiles<T, 2, kHalf ? 8 : 4, 1, B64, PAGED>(ctx, q, k, v, out, p);
         else if (nt == 3) launch_tiles<T, 3, 4, 1, B64, PAGED>(ctx, q, k, v, out, p);
-        else launch_tiles<T, 4, 4, 1, B64, PAGED>(ctx, q, k, v, out, p);
+        else launch_tiles<T, 4, 4, 1, 32, PAGED>(ctx, q, k, v, out, p);
+    } else if (kHalf && wide >= kSomeTiles) {
+        if constexpr (kHalf) {
+            if (nt == 1) launch_tiles<T, 1, 4, 4, B64, PAGED>(ctx, q, k, v, out, p);
+            else if (nt == 2) launch_tiles<T, 2, 4, 4, B64, PAGED>(ctx, q, k, v, out, p);
+            else if (nt == 3) launch_tiles<T, 3, 4, 2, B64, PAGED>(ctx, q, k, v, out, p);
+            else launch_tiles<T, 4, 4, 2, B64, PAGED>(ctx, q, k, v, out, p);
+        }
     } else {
         if (nt == 1) launch_tiles<T, 1, 1, 4, B64, PAGED>(ctx, q, k, v, out, p);
         else if (nt == 2) launch_tiles<T, 2, 1, 4, 32, PAGED>(ctx, q, k, v, out, p);
