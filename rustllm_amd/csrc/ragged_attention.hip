@@ -734,10 +734,8 @@ __global__ __launch_bounds__(64 * kSplitWaves, 2) void k_ragged_split(
 // waves: QW of 32 rows times KS shares of the key blocks, merged through LDS at
 // the end.  S^T = K Q^T leaves each lane one row's scores (32 x 32 tiles), so
 // the running max and sum need one exchange between lane halves, and the
-// probabilities come out in the operand layout of O^T += V^T P^T: for f16 with
-// keys taken in perm32 order, V's operand by transpose reads out of LDS; for
-// f32 (32x32x2 products) as they stand, V read by rows, lane i of a half
-// holding elements EC i .. + EC - 1 of it.
+// probabilities come out in the operand layout of O^T += V^T P^T, the keys taken
+// in perm32 order; V's operand comes by transpose reads out of LDS.
 // K and V go from memory straight to LDS (two stages), each lane fetching 16
 // bytes from an address of its own -- its key's row, wherever its page is --
 // the page entries read a step ahead.  Keys past the request's last read that
@@ -812,9 +810,9 @@ __device__ inline uint32_t find_tile_request(const RaggedParams& p, uint32_t u, 
 
 // Waves a SIMD that the registers leave room for: two where two workgroups of
 // four waves fit a CU's LDS.
-template <typename T, int NT, int QW, int KS, int BN>
+template <int NT, int QW, int KS, int BN>
 constexpr int kTileWaves =
-    QW * KS == 4 && BN == 32 && NT == 4 ? 3 : QW * KS == 4 && 2 * KS * 2 * BN * (NT == 3 ? 128 : 32 * NT) * int(sizeof(T)) <= 72 * 1024 ? 2 : 1;
+    QW == 4 && KS == 1 && BN == 32 && NT == 4 ? 3 : QW * KS == 4 && 2 * KS * 2 * BN * (NT == 3 ? 128 : 32 * NT) * 2 <= 72 * 1024 ? 2 : 1;
 
 // Up to 64 requests: tile u in the order of the keys that tiles see, most
 // first (in steps of a tile's tokens), so that the long ones do not start last.
@@ -854,19 +852,40 @@ __device__ inline uint32_t find_longest_tile(const RaggedParams& p, uint32_t u, 
     return uint32_t(at);
 }
 
-template <typename T, int NT, int QW, int KS, int BN, bool PAGED, bool FULL>
-__global__ __launch_bounds__(64 * QW * KS, (kTileWaves<T, NT, QW, KS, BN>)) void k_ragged_tiles(
-    const T* __restrict__ q, const T* __restrict__ k, const T* __restrict__ v,
-    T* __restrict__ out, RaggedParams p) {
-    constexpr bool kHalf = std::is_same<T, half_t>::value;
+// A workgroup's request and first row in it; false if it has none.
+template <bool PAGED>
+__device__ inline bool find_tile(const RaggedParams& p, uint32_t tile_rows, uint32_t& request,
+                                 Request& r, uint32_t& row0) {
+    const uint32_t unit = blockIdx.x / p.kv_heads;
+    uint32_t tile;
+    if (p.longest_first) {
+        request = find_longest_tile<PAGED>(p, unit, tile_rows, tile);
+        if (request >= p.sequences) return false;
+    } else {
+        const uint32_t back = gridDim.x / p.kv_heads - 1 - unit;
+        request = find_tile_request(p, back, tile_rows);
+        const uint32_t first = tiles_before(p, request, tile_rows);
+        if (back < first) return false;
+        tile = back - first;
+    }
+    r = load_request<PAGED>(p, request);
+    row0 = tile * tile_rows;
+    const uint32_t rows = r.n * p.group;
+    return uint64_t(tile) * tile_rows < rows && rows > p.small_rows;
+}
+
+template <int NT, int QW, int KS, int BN, bool PAGED, bool FULL>
+__global__ __launch_bounds__(64 * QW * KS, (kTileWaves<NT, QW, KS, BN>)) void k_ragged_tiles(
+    const half_t* __restrict__ q, const half_t* __restrict__ k, const half_t* __restrict__ v,
+    half_t* __restrict__ out, RaggedParams p) {
+    typedef half_t T;
     constexpr int D = 32 * NT;                    // head size, padded
     constexpr int RD = NT == 3 ? 128 : D;         // elements of an LDS row
-    constexpr int CE = 16 / int(sizeof(T));       // elements of a chunk
+    constexpr int CE = 8;                         // elements of a 16-byte chunk
     constexpr int ROW_CHUNKS = RD / CE;
     constexpr int SW = ROW_CHUNKS >= 16 ? 4 : ROW_CHUNKS / 4;  // lds_swizzle's row class
     constexpr int KT = BN / 32;                   // 32-key tiles of a block
     constexpr int DC = D / (2 * CE);              // pairs of chunks of a row (lane halves)
-    constexpr int EC = D / 32;                    // f32: elements of a V row a lane
     constexpr int WAVES = QW * KS;
     constexpr int THREADS = 64 * WAVES;
     constexpr uint32_t TILE = kTileRows<QW>;
@@ -884,21 +903,10 @@ __global__ __launch_bounds__(64 * QW * KS, (kTileWaves<T, NT, QW, KS, BN>)) void
 
     const uint32_t hd = FULL ? uint32_t(D) : p.head_dim;
     const uint32_t kvh = blockIdx.x % p.kv_heads;
-    const uint32_t unit = blockIdx.x / p.kv_heads;
-    uint32_t request, tile;
-    if (p.longest_first) {
-        request = find_longest_tile<PAGED>(p, unit, TILE, tile);
-        if (request >= p.sequences) return;
-    } else {
-        const uint32_t back = gridDim.x / p.kv_heads - 1 - unit;
-        request = find_tile_request(p, back, TILE);
-        tile = back - tiles_before(p, request, TILE);
-        if (back < tiles_before(p, request, TILE)) return;
-    }
-    const Request r = load_request<PAGED>(p, request);
+    uint32_t request, row0;
+    Request r;
+    if (!find_tile<PAGED>(p, TILE, request, r, row0)) return;
     const uint32_t rows = r.n * p.group;
-    if (uint64_t(tile) * TILE >= rows || rows <= p.small_rows) return;
-    const uint32_t row0 = tile * TILE;
 
     const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
     const uint32_t lane = threadIdx.x % 64;
@@ -993,42 +1001,26 @@ __global__ __launch_bounds__(64 * QW * KS, (kTileWaves<T, NT, QW, KS, BN>)) void
 
     // operands: K chunk 2 c + hs of its key's row; f16: V by transpose reads
     uint32_t koff[DC];
-    const uint32_t krow = kHalf ? perm32(col) : col;
+    const uint32_t krow = perm32(col);
 #pragma unroll
     for (int c = 0; c < DC; ++c)
         koff[c] = krow * RD * sizeof(T) + 16 * ((2 * c + hs) ^ lds_swizzle<SW>(krow));
-    constexpr int VOFFS = kHalf ? 2 * NT : 8;
-    uint32_t voff[VOFFS];
-    if constexpr (kHalf) {
+    uint32_t voff[2 * NT];
 #pragma unroll
-        for (int e2 = 0; e2 < 2; ++e2) {
-            const uint32_t vr = 8 * (lane / 32) + (lane % 16) / 4 + 4 * e2;
+    for (int e2 = 0; e2 < 2; ++e2) {
+        const uint32_t vr = 8 * (lane / 32) + (lane % 16) / 4 + 4 * e2;
 #pragma unroll
-            for (int t = 0; t < NT; ++t) {
-                const uint32_t ch = 2 * ((lane / 16) % 2) + (lane % 4) / 2 + 4 * t;
-                voff[e2 * NT + t] = vr * RD * 2 + 16 * (ch ^ lds_swizzle<SW>(vr)) + 8 * (lane % 2);
-            }
+        for (int t = 0; t < NT; ++t) {
+            const uint32_t ch = 2 * ((lane / 16) % 2) + (lane % 4) / 2 + 4 * t;
+            voff[e2 * NT + t] = vr * RD * 2 + 16 * (ch ^ lds_swizzle<SW>(vr)) + 8 * (lane % 2);
         }
-    } else {
-        // rows 8 a + 4 hs + b (a < 4, b < 4): their chunk order depends on
-        // (a % 2, b, hs); voff[4 a + b] for a < 2, two rows of eight further for a + 2
-#pragma unroll
-        for (int a = 0; a < 2; ++a)
-#pragma unroll
-            for (int b = 0; b < 4; ++b) {
-                const uint32_t vr = 8 * a + 4 * hs + b;
-                const uint32_t byte = EC * 4 * col;
-                voff[4 * a + b] =
-                    vr * RD * 4 + 16 * ((byte / 16) ^ lds_swizzle<SW>(vr)) + byte % 16;
-            }
     }
-    typedef typename std::conditional<kHalf, h8, f32x4>::type KV;
-    KV qf[DC];
+    h8 qf[DC];
     const T* qrow = q + (r.begin + token) * p.q_token + head * p.q_head + CE * hs;
 #pragma unroll
     for (int c = 0; c < DC; ++c) {
         const bool in = row_valid && (FULL || uint32_t(2 * CE * c) + CE * hs < hd);
-        qf[c] = in ? *reinterpret_cast<const KV*>(qrow + 2 * CE * c) : KV{};
+        qf[c] = in ? *reinterpret_cast<const h8*>(qrow + 2 * CE * c) : h8{};
     }
     f32x16 o[NT];
 #pragma unroll
@@ -1060,27 +1052,19 @@ __global__ __launch_bounds__(64 * QW * KS, (kTileWaves<T, NT, QW, KS, BN>)) void
                 for (int e = 0; e < 16; ++e) s[kt][e] = 0.0f;
 #pragma unroll
                 for (int c = 0; c < DC; ++c) {
-                    const KV ka = *reinterpret_cast<const KV*>(
+                    const h8 ka = *reinterpret_cast<const h8*>(
                         ks + kt * 32 * RD * sizeof(T) + koff[c]);
-                    if constexpr (kHalf) {
-                        s[kt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ka, qf[c], s[kt], 0, 0, 0);
-                    } else {
-#pragma unroll
-                        for (int e = 0; e < 4; ++e)
-                            s[kt] = __builtin_amdgcn_mfma_f32_32x32x2f32(ka[e], qf[c][e], s[kt],
-                                                                         0, 0, 0);
-                    }
+                    s[kt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ka, qf[c], s[kt], 0, 0, 0);
                 }
             }
-            // register e of tile kt: key kbase_key + 32 kt + (f16: 16 (e / 8) + 8 hs + e % 8;
-            // f32: 8 (e / 4) + 4 hs + e % 4)
+            // register e of tile kt: key kbase_key + 32 kt + 16 (e / 8) + 8 hs + e % 8
             if (kbase_key + BN > wave_least) {
-                const int lim = limit - int(kbase_key) - int((kHalf ? 8 : 4) * hs);
+                const int lim = limit - int(kbase_key) - int(8 * hs);
 #pragma unroll
                 for (int kt = 0; kt < KT; ++kt)
 #pragma unroll
                     for (int e = 0; e < 16; ++e) {
-                        const int at = 32 * kt + (kHalf ? 16 * (e / 8) + e % 8 : 8 * (e / 4) + e % 4);
+                        const int at = 32 * kt + 16 * (e / 8) + e % 8;
                         if (at > lim) s[kt][e] = -INFINITY;
                     }
             }
@@ -1104,62 +1088,29 @@ __global__ __launch_bounds__(64 * QW * KS, (kTileWaves<T, NT, QW, KS, BN>)) void
                     for (int e = 0; e < 16; ++e) o[t][e] *= alpha;
             }
             const float neg_m = m == -INFINITY ? 0.0f : -m;
-            if constexpr (kHalf) {
-                // the sum adds the same rounded probabilities that the product takes
-                const h2 ones = {half_t(1.0f), half_t(1.0f)};
-                h8 pb[BN / 16];
+            // the sum adds the same rounded probabilities that the product takes
+            const h2 ones = {half_t(1.0f), half_t(1.0f)};
+            h8 pb[BN / 16];
 #pragma unroll
-                for (int c = 0; c < BN / 16; ++c) {
+            for (int c = 0; c < BN / 16; ++c) {
 #pragma unroll
-                    for (int e = 0; e < 8; ++e)
-                        pb[c][e] = half_t(__builtin_amdgcn_exp2f(
-                            __builtin_fmaf(s[c / 2][8 * (c % 2) + e], p.scale_log2, neg_m)));
+                for (int e = 0; e < 8; ++e)
+                    pb[c][e] = half_t(__builtin_amdgcn_exp2f(
+                        __builtin_fmaf(s[c / 2][8 * (c % 2) + e], p.scale_log2, neg_m)));
 #pragma unroll
-                    for (int e = 0; e < 8; e += 2)
-                        l = __builtin_amdgcn_fdot2(h2{pb[c][e], pb[c][e + 1]}, ones, l, false);
-                }
-#pragma unroll
-                for (int c = 0; c < BN / 16; ++c)
-#pragma unroll
-                    for (int t = 0; t < NT; ++t) {
-                        const half_t* at = reinterpret_cast<const half_t*>(vs + 16 * c * RD * 2);
-                        const h4 lo = lds_read_transposed(at + voff[t] / 2);
-                        const h4 hi = lds_read_transposed(at + voff[NT + t] / 2);
-                        const h8 va = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
-                        o[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(va, pb[c], o[t], 0, 0, 0);
-                    }
-            } else {
-                typedef typename VecOf<float, EC>::type VE;
-#pragma unroll
-                for (int kt = 0; kt < KT; ++kt)
-#pragma unroll
-                    for (int e = 0; e < 16; ++e) {
-                        const float pe = __builtin_amdgcn_exp2f(
-                            __builtin_fmaf(s[kt][e], p.scale_log2, neg_m));
-                        l += pe;
-                        const int a = e / 4, b = e % 4;
-                        const unsigned char* at =
-                            vs + (32 * kt + 16 * (a / 2)) * RD * 4 + voff[4 * (a % 2) + b];
-                        float va[EC];
-                        if constexpr (EC == 3) {  // a row of 96: no 12-byte alignment to chunks
-#pragma unroll
-                            for (int t = 0; t < EC; ++t) {
-                                const uint32_t vr = 32 * kt + 8 * a + 4 * hs + b;
-                                const uint32_t byte = 4 * (EC * col + t);
-                                va[t] = *reinterpret_cast<const float*>(
-                                    vs + vr * RD * 4 + 16 * ((byte / 16) ^ lds_swizzle<SW>(vr)) +
-                                    byte % 16);
-                            }
-                        } else {
-                            const VE w = *reinterpret_cast<const VE*>(at);
-#pragma unroll
-                            for (int t = 0; t < EC; ++t) va[t] = w[t];
-                        }
-#pragma unroll
-                        for (int t = 0; t < NT; ++t)
-                            o[t] = __builtin_amdgcn_mfma_f32_32x32x2f32(va[t], pe, o[t], 0, 0, 0);
-                    }
+                for (int e = 0; e < 8; e += 2)
+                    l = __builtin_amdgcn_fdot2(h2{pb[c][e], pb[c][e + 1]}, ones, l, false);
             }
+#pragma unroll
+            for (int c = 0; c < BN / 16; ++c)
+#pragma unroll
+                for (int t = 0; t < NT; ++t) {
+                    const half_t* at = reinterpret_cast<const half_t*>(vs + 16 * c * RD * 2);
+                    const h4 lo = lds_read_transposed(at + voff[t] / 2);
+                    const h4 hi = lds_read_transposed(at + voff[NT + t] / 2);
+                    const h8 va = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+                    o[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(va, pb[c], o[t], 0, 0, 0);
+                }
         }
         __builtin_amdgcn_s_waitcnt(0);  // this wave's share of the next stage has landed
         __syncthreads();
@@ -1205,20 +1156,16 @@ __global__ __launch_bounds__(64 * QW * KS, (kTileWaves<T, NT, QW, KS, BN>)) void
         for (int t = 0; t < NT; ++t)
 #pragma unroll
             for (int g = 0; g < 4; ++g) {
-                // f16: elements 32 t + 8 g + 4 hs + 0 .. 3; f32: EC (8 g + 4 hs + i) + t
-                typename VecOf<T, 4>::type w;
+                const uint32_t d = 32 * t + 8 * g + 4 * hs;
+                if (!FULL && d >= hd) continue;
+                h4 w;
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
                     const float x = limit < 0 ? 0.0f : o[t][4 * g + i] * inv;
-                    const uint32_t d = kHalf ? 32 * t + 8 * g + 4 * hs + i
-                                             : EC * (8 * g + 4 * hs + i) + t;
-                    if (FULL || d < hd) odd |= !(fabsf(x) < INFINITY);
-                    w[i] = r.bad ? T(NAN) : from_float<T>(x);
-                    if (!kHalf && (FULL || d < hd)) orow[d] = w[i];
+                    odd |= !(fabsf(x) < INFINITY);
+                    w[i] = r.bad ? half_t(NAN) : half_t(x);
                 }
-                const uint32_t d = 32 * t + 8 * g + 4 * hs;
-                if (kHalf && (FULL || d < hd))
-                    *reinterpret_cast<typename VecOf<T, 4>::type*>(orow + d) = w;
+                *reinterpret_cast<h4*>(orow + d) = w;
             }
     }
     if (r.bad) return;
@@ -1232,6 +1179,304 @@ __global__ __launch_bounds__(64 * QW * KS, (kTileWaves<T, NT, QW, KS, BN>)) void
         const uint32_t again = wrow0 + __builtin_ctz(redo);
         row_by_wave<T, PAGED>(q, k, v, out, p, request, r, again / p.group,
                               kvh * p.group + again % p.group);
+    }
+}
+
+// ------------------------------------- many rows per KV head, f32 products
+//
+// The same tiles with every f32 operand as three bf16 parts (Bf16x3: six of the
+// nine products, the rest below 2^-26 of the whole), at 6/16 of the f16 rate
+// against 1/16 for f32 products of the matrix cores.  A block is 32 keys of one
+// wave, and nothing passes through LDS: K's operand is 32 bytes of a key's row
+// a lane; V's comes by columns, so a lane loads its NT elements of eight
+// neighbouring rows and splits each column across them.  K's registers are
+// refilled once the scores are through, V's after the products.
+//
+// Queries, probabilities and values are scaled by 2^24 (kPartScale) so that no
+// part of theirs falls below bf16's range; of a key only what is below 2^-126
+// is lost, which changes a score by less than 2^-59 while query elements are
+// below 2^60.  Rows with larger query elements, and rows whose output is not
+// finite (infinities, sums of 2^80 and more), are computed again unsplit
+// (row_by_wave).
+template <int NT, int QW, int KS, bool PAGED, bool FULL>
+__global__ __launch_bounds__(64 * QW * KS, NT <= 2 ? 2 : 1) void k_ragged_tiles_f32(
+    const float* __restrict__ q, const float* __restrict__ k, const float* __restrict__ v,
+    float* __restrict__ out, RaggedParams p) {
+    constexpr int D = 32 * NT;
+    constexpr int DC = D / 16;
+    constexpr uint32_t BN = 32;
+    constexpr uint32_t TILE = kTileRows<QW>;
+    constexpr int MERGE = NT * 16 + 2;
+    __shared__ float merge[KS > 1 ? (KS - 1) * QW * 64 * MERGE : 1];
+    __shared__ uint32_t any_bad;
+
+    const uint32_t hd = FULL ? uint32_t(D) : p.head_dim;
+    const uint32_t kvh = blockIdx.x % p.kv_heads;
+    uint32_t request, row0;
+    Request r;
+    if (!find_tile<PAGED>(p, TILE, request, r, row0)) return;
+    const uint32_t rows = r.n * p.group;
+    const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
+    const uint32_t lane = threadIdx.x % 64;
+    const uint32_t qw = wave % QW, share = wave / QW;
+    const uint32_t col = lane % 32, hs = lane / 32;
+    const uint32_t last = r.keys == 0 ? 0u : r.keys - 1;
+    auto keys_of = [&](uint32_t row) {  // visible to row `row` of the request
+        const int64_t pos = r.first + row / p.group;
+        return pos < 0 || r.bad ? 0u : uint32_t(min(int64_t(r.keys), pos + 1));
+    };
+    const uint32_t wrow0 = row0 + 32 * qw;
+    const bool wave_active = wrow0 < rows;
+    const uint32_t wave_keys = wave_active ? keys_of(min(wrow0 + 31, rows - 1)) : 0u;
+    const uint32_t wave_least = wave_active ? keys_of(wrow0) : 0u;
+    const uint32_t blocks = (wave_keys + BN - 1) / BN;
+    const uint32_t row = wrow0 + col;
+    const bool row_valid = row < rows;
+    const uint32_t token = row_valid ? row / p.group : 0u;
+    const uint32_t head = kvh * p.group + (row_valid ? row % p.group : 0u);
+    const int limit = row_valid ? int(keys_of(row)) - 1 : -1;
+    if (threadIdx.x == 0) any_bad = 0;
+
+    const uint32_t* entries = PAGED ? p.table + uint64_t(request) * p.max_blocks : nullptr;
+    const uint32_t mask = (1u << p.shift) - 1;
+    const char* kbase;
+    const char* vbase;
+    uint32_t k_row_bytes, v_row_bytes;  // between the rows of a page, or of a request
+    if constexpr (PAGED) {
+        kbase = reinterpret_cast<const char*>(k) + uint64_t(kvh) * p.head_bytes;
+        vbase = reinterpret_cast<const char*>(v) + uint64_t(kvh) * p.head_bytes;
+        k_row_bytes = v_row_bytes = hd * 4;
+    } else {
+        kbase = reinterpret_cast<const char*>(k + r.begin * p.k_token + kvh * p.k_head);
+        vbase = reinterpret_cast<const char*>(v + r.begin * p.v_token + kvh * p.v_head);
+        k_row_bytes = uint32_t(p.k_token * 4);
+        v_row_bytes = uint32_t(p.v_token * 4);
+    }
+    bool bad_page = false;
+    struct Entries {
+        uint32_t k, v[2];
+    };
+    auto load_entries = [&](uint32_t blk) {  // of this lane's K row and its two runs of V rows
+        Entries e{};
+        if constexpr (PAGED) {
+            e.k = entries[min(blk * BN + perm32(col), last) >> p.shift];
+#pragma unroll
+            for (int c = 0; c < 2; ++c)
+                e.v[c] = entries[min(blk * BN + 16 * c + 8 * hs, last) >> p.shift];
+        }
+        return e;
+    };
+    auto page_at = [&](const char* base, uint32_t entry) {
+        if constexpr (!PAGED) return base;
+        const bool in = entry < p.pages;
+        bad_page |= !in;
+        return base + uint64_t(in ? entry : 0u) * p.page_bytes;
+    };
+    f32x8 kreg[DC];
+    float vreg[2][8][NT];
+    auto load_keys = [&](uint32_t blk, const Entries& e) {
+        const uint32_t key = min(blk * BN + perm32(col), last);
+        const char* at = page_at(kbase, e.k) +
+                         uint64_t(PAGED ? key & mask : key) * k_row_bytes + 32 * hs;
+#pragma unroll
+        for (int c = 0; c < DC; ++c) {
+            f32x4 x[2];
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                const bool in = FULL || uint32_t(16 * c + 8 * hs + 4 * i) < hd;
+                x[i] = in ? *reinterpret_cast<const f32x4*>(at + 64 * c + 16 * i) : f32x4{};
+            }
+            kreg[c] = __builtin_shufflevector(x[0], x[1], 0, 1, 2, 3, 4, 5, 6, 7);
+        }
+    };
+    auto load_values = [&](uint32_t blk, const Entries& e) {
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+            const uint32_t run = blk * BN + 16 * c + 8 * hs;  // eight keys inside one page
+            const char* base = page_at(vbase, e.v[c]);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const uint32_t key = min(run + i, last);
+                const char* at = base + uint64_t(PAGED ? key & mask : key) * v_row_bytes;
+                if constexpr (NT == 3) {  // element 32 t + col
+#pragma unroll
+                    for (int t = 0; t < NT; ++t) {
+                        const uint32_t d = 32 * t + col;
+                        vreg[c][i][t] =
+                            *reinterpret_cast<const float*>(at + 4 * (FULL || d < hd ? d : 0u));
+                    }
+                } else {  // elements NT col .. + NT - 1
+                    typedef typename VecOf<float, NT>::type VE;
+                    const uint32_t d = NT * col;
+                    const VE w = *reinterpret_cast<const VE*>(at + 4 * (FULL || d < hd ? d : 0u));
+#pragma unroll
+                    for (int t = 0; t < NT; ++t) vreg[c][i][t] = w[t];
+                }
+            }
+        }
+    };
+    uint32_t blk = share;
+    Entries e = load_entries(blk);
+    if (blk < blocks) {
+        load_keys(blk, e);
+        load_values(blk, e);
+    }
+
+    Bf16x3 qf[DC];
+    float widest = 0.0f;  // query element
+    const float* qrow = q + (r.begin + token) * p.q_token + head * p.q_head + 8 * hs;
+#pragma unroll
+    for (int c = 0; c < DC; ++c) {
+        f32x8 x;
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const bool in = row_valid && (FULL || uint32_t(16 * c + 8 * hs + 4 * i) < hd);
+            const f32x4 w = in ? *reinterpret_cast<const f32x4*>(qrow + 16 * c + 4 * i) : f32x4{};
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                widest = fmaxf(widest, fabsf(w[j]));
+                x[4 * i + j] = w[j] * kPartScale;
+            }
+        }
+        qf[c] = split_bf16(x);
+    }
+    const float scale_log2 = p.scale_log2 / kPartScale;  // of the scores, their queries scaled
+    f32x16 o[NT];
+#pragma unroll
+    for (int t = 0; t < NT; ++t)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) o[t][i] = 0.0f;
+    float m = -INFINITY, l = 0.0f;
+
+    if (PAGED && blk + KS < blocks) e = load_entries(blk + KS);
+    for (; blk < blocks; blk += KS) {
+        const bool more = blk + KS < blocks;
+        f32x16 s;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) s[i] = 0.0f;
+#pragma unroll
+        for (int c = 0; c < DC; ++c) s = mfma_bf16x3(split_bf16(kreg[c]), qf[c], s);
+        if (more) load_keys(blk + KS, e);
+        // register i: key blk BN + 16 (i / 8) + 8 hs + i % 8
+        if (blk * BN + BN > wave_least) {
+            const int lim = limit - int(blk * BN) - int(8 * hs);
+#pragma unroll
+            for (int i = 0; i < 16; ++i)
+                if (16 * (i / 8) + i % 8 > lim) s[i] = -INFINITY;
+        }
+        float mx = -INFINITY, my = -INFINITY;
+#pragma unroll
+        for (int i = 0; i < 16; i += 4) {
+            mx = max3(mx, s[i], s[i + 1]);
+            my = max3(my, s[i + 2], s[i + 3]);
+        }
+        mx = halves_max(fmaxf(mx, my)) * scale_log2;
+        if (__any(mx > m + kSlack)) {
+            const float m_new = fmaxf(m, mx);
+            const float alpha = m_new > m ? __builtin_amdgcn_exp2f(m - m_new) : 1.0f;
+            m = m_new;
+            l *= alpha;
+#pragma unroll
+            for (int t = 0; t < NT; ++t)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) o[t][i] *= alpha;
+        }
+        const float neg_m = m == -INFINITY ? 0.0f : -m;
+        Bf16x3 pb[2];
+        float la = 0.0f, lb = 0.0f;
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+            f32x8 x;
+#pragma unroll
+            for (int i = 0; i < 8; i += 2) {
+                x[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[8 * c + i], scale_log2, neg_m));
+                x[i + 1] =
+                    __builtin_amdgcn_exp2f(__builtin_fmaf(s[8 * c + i + 1], scale_log2, neg_m));
+                la += x[i];
+                lb += x[i + 1];
+            }
+            pb[c] = split_bf16(x * kPartScale);
+        }
+        l += la + lb;
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+            // the block's products apart, added to the output once
+            f32x16 acc;
+#pragma unroll
+            for (int i = 0; i < 16; ++i) acc[i] = 0.0f;
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+                f32x8 x;
+#pragma unroll
+                for (int i = 0; i < 8; ++i) x[i] = vreg[c][i][t] * kPartScale;
+                acc = mfma_bf16x3(split_bf16(x), pb[c], acc);
+            }
+#pragma unroll
+            for (int i = 0; i < 16; ++i) o[t][i] += acc[i];
+        }
+        if (more) {
+            load_values(blk + KS, e);
+            if (PAGED && blk + 2 * KS < blocks) e = load_entries(blk + 2 * KS);
+        }
+    }
+    if constexpr (KS > 1 || PAGED) __syncthreads();  // any_bad is set up
+    if (PAGED && __any(bad_page) && lane == 0) any_bad = 1;
+
+    if constexpr (KS > 1) {
+        if (share > 0) {
+            float* dst = merge + ((share - 1) * QW * 64 + qw * 64 + lane) * MERGE;
+            dst[0] = m;
+            dst[1] = l;
+#pragma unroll
+            for (int t = 0; t < NT; ++t)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) dst[2 + 16 * t + i] = o[t][i];
+        }
+        __syncthreads();
+        if (share != 0) return;
+#pragma unroll
+        for (int x = 1; x < KS; ++x) {
+            const float* src = merge + ((x - 1) * QW * 64 + qw * 64 + lane) * MERGE;
+            const float m2 = src[0], top = fmaxf(m, m2);
+            const float a1 = top > m ? __builtin_amdgcn_exp2f(m - top) : 1.0f;
+            const float a2 = top > m2 ? __builtin_amdgcn_exp2f(m2 - top) : 1.0f;
+            l = l * a1 + src[1] * a2;
+#pragma unroll
+            for (int t = 0; t < NT; ++t)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) o[t][i] = o[t][i] * a1 + src[2 + 16 * t + i] * a2;
+            m = top;
+        }
+    } else if (PAGED) {
+        __syncthreads();
+    }
+
+    const float inv = kProductUnscale / (l + __shfl_xor(l, 32, 64));
+    bool odd = (PAGED && any_bad != 0) || widest >= 0x1p60f;
+    if (row_valid) {
+        float* orow = out + (uint64_t(r.begin + token) * p.q_heads + head) * hd;
+#pragma unroll
+        for (int t = 0; t < NT; ++t)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                // the tile's row, and its element
+                const uint32_t at = 8 * (i / 4) + 4 * hs + i % 4;
+                const uint32_t d = NT == 3 ? 32 * t + at : NT * at + t;
+                if (!FULL && d >= hd) continue;
+                const float x = limit < 0 ? 0.0f : o[t][i] * inv;
+                odd |= !(fabsf(x) < INFINITY);
+                orow[d] = r.bad ? NAN : x;
+            }
+    }
+    if (r.bad) return;
+    const uint64_t votes = __ballot(odd && row_valid);
+    uint32_t redo = uint32_t(votes | votes >> 32);
+    if (redo == 0) return;
+    __builtin_amdgcn_s_waitcnt(0);
+    for (; redo != 0; redo &= redo - 1) {
+        const uint32_t again = wrow0 + __builtin_ctz(redo);
+        row_by_wave<float, PAGED>(q, k, v, out, p, request, r, again / p.group,
+                                  kvh * p.group + again % p.group);
     }
 }
 
@@ -1288,48 +1533,64 @@ void launch_rows(rl_context* ctx, const T* q, const T* k, const T* v, T* out,
         RL_LAUNCH(ctx, (k_ragged_rows<T, 8, PAGED>), grid, block, q, k, v, out, p);
 }
 
-constexpr uint64_t kManyTiles = 1;
-constexpr uint64_t kSomeTiles = 1000000;
-// The tile kernel for a batch of at most `tokens` rows.
+// The tile kernels for a batch of at most `tokens` rows.
 template <typename T, int NT, int QW, int KS, int BN, bool PAGED>
 void launch_tiles(rl_context* ctx, const T* q, const T* k, const T* v, T* out,
                   const RaggedParams& p) {
     const uint64_t units =
         uint64_t(p.tokens) * p.group / kTileRows<QW> + p.sequences;
     const dim3 grid(uint32_t(units * p.kv_heads)), block(64 * QW * KS);
-    if (p.head_dim == 32 * NT)
-        RL_LAUNCH(ctx, (k_ragged_tiles<T, NT, QW, KS, BN, PAGED, true>), grid, block, q, k, v, out,
-                  p);
-    else
-        RL_LAUNCH(ctx, (k_ragged_tiles<T, NT, QW, KS, BN, PAGED, false>), grid, block, q, k, v,
-                  out, p);
+    const bool full = p.head_dim == 32 * NT;
+    if constexpr (std::is_same<T, float>::value) {
+        if (full)
+            RL_LAUNCH(ctx, (k_ragged_tiles_f32<NT, QW, KS, PAGED, true>), grid, block, q, k, v,
+                      out, p);
+        else
+            RL_LAUNCH(ctx, (k_ragged_tiles_f32<NT, QW, KS, PAGED, false>), grid, block, q, k, v,
+                      out, p);
+    } else {
+        if (full)
+            RL_LAUNCH(ctx, (k_ragged_tiles<NT, QW, KS, BN, PAGED, true>), grid, block, q, k, v,
+                      out, p);
+        else
+            RL_LAUNCH(ctx, (k_ragged_tiles<NT, QW, KS, BN, PAGED, false>), grid, block, q, k, v,
+                      out, p);
+    }
 }
 template <typename T, bool PAGED>
 void launch_tiles(rl_context* ctx, const T* q, const T* k, const T* v, T* out, RaggedParams p) {
     constexpr bool kHalf = std::is_same<T, half_t>::value;
-    const uint64_t wide =
-        (uint64_t(p.tokens) * p.group / kTileRows<4>) * p.kv_heads;
+    const uint64_t cus = uint64_t(ctx->num_cus);
+    const uint64_t wide = (uint64_t(p.tokens) * p.group / kTileRows<4>) * p.kv_heads;
     const uint32_t nt = (p.head_dim + 31) / 32;
-    const uint64_t slots = (nt <= 2 ? 4 : 2) * uint64_t(ctx->num_cus);  // wide tiles at once
+    const uint64_t slots = (nt <= 2 ? 4 : 2) * cus;  // wide tiles at once
     p.longest_first = p.sequences <= 64 && wide >= slots && wide <= 3 * slots;
-    constexpr int B64 = kHalf ? 64 : 32;  // keys of a block: 8 KB of K for 64 elements a row
-    if (wide >= kManyTiles * uint64_t(ctx->num_cus)) {
-        if (nt == 1) launch_tiles<T, 1, 4, 1, B64, PAGED>(ctx, q, k, v, out, p);
-        else if (nt == 2) launch_tiles<T, 2, kHalf ? 8 : 4, 1, B64, PAGED>(ctx, q, k, v, out, p);
-        else if (nt == 3) launch_tiles<T, 3, 4, 1, B64, PAGED>(ctx, q, k, v, out, p);
-        else launch_tiles<T, 4, 4, 1, 32, PAGED>(ctx, q, k, v, out, p);
-    } else if (kHalf && wide >= kSomeTiles) {
-        if constexpr (kHalf) {
-            if (nt == 1) launch_tiles<T, 1, 4, 4, B64, PAGED>(ctx, q, k, v, out, p);
-            else if (nt == 2) launch_tiles<T, 2, 4, 4, B64, PAGED>(ctx, q, k, v, out, p);
-            else if (nt == 3) launch_tiles<T, 3, 4, 2, B64, PAGED>(ctx, q, k, v, out, p);
-            else launch_tiles<T, 4, 4, 2, B64, PAGED>(ctx, q, k, v, out, p);
+    if constexpr (kHalf) {
+        if (wide >= cus) {
+            if (nt == 1) launch_tiles<T, 1, 4, 1, 64, PAGED>(ctx, q, k, v, out, p);
+            else if (nt == 2) launch_tiles<T, 2, 8, 1, 64, PAGED>(ctx, q, k, v, out, p);
+            else if (nt == 3) launch_tiles<T, 3, 4, 1, 64, PAGED>(ctx, q, k, v, out, p);
+            else launch_tiles<T, 4, 4, 1, 32, PAGED>(ctx, q, k, v, out, p);
+        } else {
+            if (nt == 1) launch_tiles<T, 1, 2, 2, 64, PAGED>(ctx, q, k, v, out, p);
+            else if (nt == 2) launch_tiles<T, 2, 2, 2, 64, PAGED>(ctx, q, k, v, out, p);
+            else if (nt == 3) launch_tiles<T, 3, 2, 2, 32, PAGED>(ctx, q, k, v, out, p);
+            else launch_tiles<T, 4, 2, 2, 32, PAGED>(ctx, q, k, v, out, p);
         }
     } else {
-        if (nt == 1) launch_tiles<T, 1, 1, 4, B64, PAGED>(ctx, q, k, v, out, p);
-        else if (nt == 2) launch_tiles<T, 2, 1, 4, 32, PAGED>(ctx, q, k, v, out, p);
-        else if (nt == 3) launch_tiles<T, 3, 1, 2, 32, PAGED>(ctx, q, k, v, out, p);
-        else launch_tiles<T, 4, 1, 2, 32, PAGED>(ctx, q, k, v, out, p);
+        p.longest_first = p.sequences <= 64 && wide < 4 * cus;
+        if (nt >= 3 && wide >= cus) {
+            if (nt == 3) launch_tiles<T, 3, 4, 1, 32, PAGED>(ctx, q, k, v, out, p);
+            else launch_tiles<T, 4, 4, 1, 32, PAGED>(ctx, q, k, v, out, p);
+        } else if (wide >= cus) {
+            if (nt == 1) launch_tiles<T, 1, 2, 2, 32, PAGED>(ctx, q, k, v, out, p);
+            else launch_tiles<T, 2, 2, 2, 32, PAGED>(ctx, q, k, v, out, p);
+        } else {
+            if (nt == 1) launch_tiles<T, 1, 1, 4, 32, PAGED>(ctx, q, k, v, out, p);
+            else if (nt == 2) launch_tiles<T, 2, 1, 4, 32, PAGED>(ctx, q, k, v, out, p);
+            else if (nt == 3) launch_tiles<T, 3, 1, 4, 32, PAGED>(ctx, q, k, v, out, p);
+            else launch_tiles<T, 4, 1, 4, 32, PAGED>(ctx, q, k, v, out, p);
+        }
     }
 }
 
