@@ -360,10 +360,16 @@ __device__ inline uint32_t last_lane(uint32_t v) {
 // FULL: the head size is DP; else it is a smaller multiple of 16 bytes and the
 // operands' elements past it are zeros (K, Q) or any row's own (V, whose output
 // columns are not stored).
+template <int DP>
+struct SplitLds {
+    float ml[kSplitWaves][kSplitRows][2];
+    float o[kSplitWaves][kSplitRows][DP + 4];
+    uint32_t odd_rows, ticket;
+};
 template <typename T, int DP, bool FULL>
-__global__ __launch_bounds__(64 * kSplitWaves, 2) void k_ragged_split(
-    const T* __restrict__ q, const T* __restrict__ k, const T* __restrict__ v,
-    T* __restrict__ out, RaggedParams p) {
+__device__ inline void split_rows(const T* __restrict__ q, const T* __restrict__ k,
+                                  const T* __restrict__ v, T* __restrict__ out,
+                                  const RaggedParams& p, SplitLds<DP>& lds, uint32_t block) {
     typedef SplitShape<T, DP> S;
     typedef SplitBlock<T, DP> Block;
     typedef typename Block::KV KV;
@@ -372,15 +378,16 @@ __global__ __launch_bounds__(64 * kSplitWaves, 2) void k_ragged_split(
     constexpr uint32_t kKeys = S::kKeys;
     constexpr uint32_t kUnit = kSplitWaves * kKeys;
     constexpr uint32_t kUnitShift = __builtin_ctz(kUnit);
-    __shared__ float merge_ml[kSplitWaves][kSplitRows][2];
-    __shared__ __align__(16) float merge_o[kSplitWaves][kSplitRows][DP + 4];
-    __shared__ uint32_t odd_rows, ticket;
+    auto& merge_ml = lds.ml;
+    auto& merge_o = lds.o;
+    uint32_t& odd_rows = lds.odd_rows;
+    uint32_t& ticket = lds.ticket;
     const uint32_t hd = FULL ? uint32_t(DP) : p.head_dim;
     const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
     const uint32_t lane = threadIdx.x % 64;
     const uint32_t lr = lane % 16, g = lane / 16;
-    const uint32_t kvh = blockIdx.x % p.kv_heads;
-    const uint64_t w = blockIdx.x / p.kv_heads;
+    const uint32_t kvh = block % p.kv_heads;
+    const uint64_t w = block / p.kv_heads;
 
     // Every workgroup's share of the units: `per` of them in request order.
     Request lane0;  // of the first 64 requests
@@ -854,15 +861,16 @@ __device__ inline uint32_t find_longest_tile(const RaggedParams& p, uint32_t u, 
 
 // A workgroup's request and first row in it; false if it has none.
 template <bool PAGED>
-__device__ inline bool find_tile(const RaggedParams& p, uint32_t tile_rows, uint32_t& request,
-                                 Request& r, uint32_t& row0) {
-    const uint32_t unit = blockIdx.x / p.kv_heads;
+__device__ inline bool find_tile(const RaggedParams& p, uint32_t block, uint32_t blocks,
+                                 uint32_t tile_rows, uint32_t& request, Request& r,
+                                 uint32_t& row0) {
+    const uint32_t unit = block / p.kv_heads;
     uint32_t tile;
     if (p.longest_first) {
         request = find_longest_tile<PAGED>(p, unit, tile_rows, tile);
         if (request >= p.sequences) return false;
     } else {
-        const uint32_t back = gridDim.x / p.kv_heads - 1 - unit;
+        const uint32_t back = blocks / p.kv_heads - 1 - unit;
         request = find_tile_request(p, back, tile_rows);
         const uint32_t first = tiles_before(p, request, tile_rows);
         if (back < first) return false;
@@ -874,10 +882,20 @@ __device__ inline bool find_tile(const RaggedParams& p, uint32_t tile_rows, uint
     return uint64_t(tile) * tile_rows < rows && rows > p.small_rows;
 }
 
+// LDS of a tile: two stages of every share's K and V blocks, then the merge.
+template <int NT, int QW, int KS, int BN>
+struct TileLds {
+    static constexpr int kRow = NT == 3 ? 128 : 32 * NT;  // elements of a row
+    static constexpr int kStages = 2 * KS * 2 * BN * kRow * 2;
+    static constexpr int kMerge = (KS - 1) * QW * 64 * (NT * 16 + 2) * 4;
+    unsigned char bytes[kStages > kMerge ? kStages : kMerge];
+    uint32_t any_bad;
+};
 template <int NT, int QW, int KS, int BN, bool PAGED, bool FULL>
-__global__ __launch_bounds__(64 * QW * KS, (kTileWaves<NT, QW, KS, BN>)) void k_ragged_tiles(
-    const half_t* __restrict__ q, const half_t* __restrict__ k, const half_t* __restrict__ v,
-    half_t* __restrict__ out, RaggedParams p) {
+__device__ inline void tile_rows(const half_t* __restrict__ q, const half_t* __restrict__ k,
+                                 const half_t* __restrict__ v, half_t* __restrict__ out,
+                                 const RaggedParams& p, TileLds<NT, QW, KS, BN>& shared,
+                                 uint32_t block, uint32_t n_blocks) {
     typedef half_t T;
     constexpr int D = 32 * NT;                    // head size, padded
     constexpr int RD = NT == 3 ? 128 : D;         // elements of an LDS row
@@ -894,18 +912,16 @@ __global__ __launch_bounds__(64 * QW * KS, (kTileWaves<NT, QW, KS, BN>)) void k_
     constexpr int BLOCK_BYTES = 16 * BLOCK_CHUNKS;
     constexpr int STAGE_BYTES = KS * 2 * BLOCK_BYTES;
     constexpr int MERGE = NT * 16 + 2;
-    constexpr int MERGE_BYTES = (KS - 1) * QW * 64 * MERGE * 4;
-    constexpr int LDS_BYTES = 2 * STAGE_BYTES > MERGE_BYTES ? 2 * STAGE_BYTES : MERGE_BYTES;
     static_assert(BLOCK_CHUNKS % 64 == 0 && BLOCK_CHUNKS * KS % THREADS == 0,
                   "a wave's load stays in one block");
-    __shared__ __align__(16) unsigned char lds[LDS_BYTES];
-    __shared__ uint32_t any_bad;
+    unsigned char* const lds = shared.bytes;
+    uint32_t& any_bad = shared.any_bad;
 
     const uint32_t hd = FULL ? uint32_t(D) : p.head_dim;
-    const uint32_t kvh = blockIdx.x % p.kv_heads;
+    const uint32_t kvh = block % p.kv_heads;
     uint32_t request, row0;
     Request r;
-    if (!find_tile<PAGED>(p, TILE, request, r, row0)) return;
+    if (!find_tile<PAGED>(p, block, n_blocks, TILE, request, r, row0)) return;
     const uint32_t rows = r.n * p.group;
 
     const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
@@ -1198,23 +1214,29 @@ __global__ __launch_bounds__(64 * QW * KS, (kTileWaves<NT, QW, KS, BN>)) void k_
 // below 2^60.  Rows with larger query elements, and rows whose output is not
 // finite (infinities, sums of 2^80 and more), are computed again unsplit
 // (row_by_wave).
+template <int NT, int QW, int KS>
+struct TileLdsF32 {
+    float merge[KS > 1 ? (KS - 1) * QW * 64 * (NT * 16 + 2) : 1];
+    uint32_t any_bad;
+};
 template <int NT, int QW, int KS, bool PAGED, bool FULL>
-__global__ __launch_bounds__(64 * QW * KS, NT <= 2 ? 2 : 1) void k_ragged_tiles_f32(
-    const float* __restrict__ q, const float* __restrict__ k, const float* __restrict__ v,
-    float* __restrict__ out, RaggedParams p) {
+__device__ inline void tile_rows_f32(const float* __restrict__ q, const float* __restrict__ k,
+                                     const float* __restrict__ v, float* __restrict__ out,
+                                     const RaggedParams& p, TileLdsF32<NT, QW, KS>& shared,
+                                     uint32_t block, uint32_t n_blocks) {
     constexpr int D = 32 * NT;
     constexpr int DC = D / 16;
     constexpr uint32_t BN = 32;
     constexpr uint32_t TILE = kTileRows<QW>;
     constexpr int MERGE = NT * 16 + 2;
-    __shared__ float merge[KS > 1 ? (KS - 1) * QW * 64 * MERGE : 1];
-    __shared__ uint32_t any_bad;
+    float* const merge = shared.merge;
+    uint32_t& any_bad = shared.any_bad;
 
     const uint32_t hd = FULL ? uint32_t(D) : p.head_dim;
-    const uint32_t kvh = blockIdx.x % p.kv_heads;
+    const uint32_t kvh = block % p.kv_heads;
     uint32_t request, row0;
     Request r;
-    if (!find_tile<PAGED>(p, TILE, request, r, row0)) return;
+    if (!find_tile<PAGED>(p, block, n_blocks, TILE, request, r, row0)) return;
     const uint32_t rows = r.n * p.group;
     const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
     const uint32_t lane = threadIdx.x % 64;
@@ -1480,6 +1502,72 @@ __global__ __launch_bounds__(64 * QW * KS, NT <= 2 ? 2 : 1) void k_ragged_tiles_
     }
 }
 
+// ----------------------------------------------------------------- kernels
+
+template <typename T, int DP, bool FULL>
+__global__ __launch_bounds__(64 * kSplitWaves, 2) void k_ragged_split(
+    const T* __restrict__ q, const T* __restrict__ k, const T* __restrict__ v,
+    T* __restrict__ out, RaggedParams p) {
+    __shared__ __align__(16) SplitLds<DP> lds;
+    split_rows<T, DP, FULL>(q, k, v, out, p, lds, blockIdx.x);
+}
+
+// A tile's LDS and body by type.
+template <typename T, int NT, int QW, int KS, int BN>
+struct Tile {
+    typedef TileLds<NT, QW, KS, BN> Lds;
+    static constexpr int kWaves = kTileWaves<NT, QW, KS, BN>;
+    template <bool PAGED, bool FULL>
+    __device__ static inline void run(const T* q, const T* k, const T* v, T* out,
+                                      const RaggedParams& p, Lds& lds, uint32_t block,
+                                      uint32_t blocks) {
+        tile_rows<NT, QW, KS, BN, PAGED, FULL>(q, k, v, out, p, lds, block, blocks);
+    }
+};
+template <int NT, int QW, int KS, int BN>
+struct Tile<float, NT, QW, KS, BN> {
+    typedef TileLdsF32<NT, QW, KS> Lds;
+    static constexpr int kWaves = NT <= 2 ? 2 : 1;
+    template <bool PAGED, bool FULL>
+    __device__ static inline void run(const float* q, const float* k, const float* v, float* out,
+                                      const RaggedParams& p, Lds& lds, uint32_t block,
+                                      uint32_t blocks) {
+        tile_rows_f32<NT, QW, KS, PAGED, FULL>(q, k, v, out, p, lds, block, blocks);
+    }
+};
+
+template <typename T, int NT, int QW, int KS, int BN, bool FULL>
+__global__ __launch_bounds__(64 * QW * KS, (Tile<T, NT, QW, KS, BN>::kWaves)) void k_packed_tiles(
+    const T* __restrict__ q, const T* __restrict__ k, const T* __restrict__ v,
+    T* __restrict__ out, RaggedParams p) {
+    typedef Tile<T, NT, QW, KS, BN> Body;
+    __shared__ __align__(16) typename Body::Lds lds;
+    Body::template run<false, FULL>(q, k, v, out, p, lds, blockIdx.x, gridDim.x);
+}
+
+// A paged batch of chunks and single tokens in one launch: the first
+// split_blocks workgroups stream the keys of the requests of few rows, the
+// others take tiles, so that the one's wait for memory runs beside the other's
+// products.
+template <typename T, int NT, int QW, int KS, int BN, bool FULL>
+__global__ __launch_bounds__(64 * QW * KS, (Tile<T, NT, QW, KS, BN>::kWaves)) void k_paged_mixed(
+    const T* __restrict__ q, const T* __restrict__ k, const T* __restrict__ v,
+    T* __restrict__ out, RaggedParams p, uint32_t split_blocks) {
+    static_assert(QW * KS == kSplitWaves, "both parts take four waves");
+    typedef Tile<T, NT, QW, KS, BN> Body;
+    constexpr int DP = NT <= 2 ? 64 : 128;
+    union Lds {
+        typename Body::Lds tile;
+        SplitLds<DP> split;
+    };
+    __shared__ __align__(16) Lds lds;
+    if (blockIdx.x < split_blocks)
+        split_rows<T, DP, FULL && 32 * NT == DP>(q, k, v, out, p, lds.split, blockIdx.x);
+    else
+        Body::template run<true, FULL>(q, k, v, out, p, lds.tile, blockIdx.x - split_blocks,
+                                       gridDim.x - split_blocks);
+}
+
 // -------------------------------------------------------------- workspace
 //
 // The split kernel's workgroups (two fit a CU: registers), their partials and
@@ -1533,63 +1621,72 @@ void launch_rows(rl_context* ctx, const T* q, const T* k, const T* v, T* out,
         RL_LAUNCH(ctx, (k_ragged_rows<T, 8, PAGED>), grid, block, q, k, v, out, p);
 }
 
-// The tile kernels for a batch of at most `tokens` rows.
+// The tile kernels for a batch of at most `tokens` rows; paged ones with
+// `split_blocks` workgroups for the requests of few rows.
 template <typename T, int NT, int QW, int KS, int BN, bool PAGED>
 void launch_tiles(rl_context* ctx, const T* q, const T* k, const T* v, T* out,
-                  const RaggedParams& p) {
+                  const RaggedParams& p, uint32_t split_blocks) {
     const uint64_t units =
         uint64_t(p.tokens) * p.group / kTileRows<QW> + p.sequences;
-    const dim3 grid(uint32_t(units * p.kv_heads)), block(64 * QW * KS);
+    const dim3 grid(uint32_t(units * p.kv_heads) + split_blocks), block(64 * QW * KS);
     const bool full = p.head_dim == 32 * NT;
-    if constexpr (std::is_same<T, float>::value) {
+    if constexpr (PAGED) {
         if (full)
-            RL_LAUNCH(ctx, (k_ragged_tiles_f32<NT, QW, KS, PAGED, true>), grid, block, q, k, v,
-                      out, p);
+            RL_LAUNCH(ctx, (k_paged_mixed<T, NT, QW, KS, BN, true>), grid, block, q, k, v, out, p,
+                      split_blocks);
         else
-            RL_LAUNCH(ctx, (k_ragged_tiles_f32<NT, QW, KS, PAGED, false>), grid, block, q, k, v,
-                      out, p);
+            RL_LAUNCH(ctx, (k_paged_mixed<T, NT, QW, KS, BN, false>), grid, block, q, k, v, out,
+                      p, split_blocks);
     } else {
         if (full)
-            RL_LAUNCH(ctx, (k_ragged_tiles<NT, QW, KS, BN, PAGED, true>), grid, block, q, k, v,
-                      out, p);
+            RL_LAUNCH(ctx, (k_packed_tiles<T, NT, QW, KS, BN, true>), grid, block, q, k, v, out,
+                      p);
         else
-            RL_LAUNCH(ctx, (k_ragged_tiles<NT, QW, KS, BN, PAGED, false>), grid, block, q, k, v,
-                      out, p);
+            RL_LAUNCH(ctx, (k_packed_tiles<T, NT, QW, KS, BN, false>), grid, block, q, k, v, out,
+                      p);
     }
 }
+constexpr uint64_t kSomeTiles = 100;
 template <typename T, bool PAGED>
-void launch_tiles(rl_context* ctx, const T* q, const T* k, const T* v, T* out, RaggedParams p) {
+void launch_tiles(rl_context* ctx, const T* q, const T* k, const T* v, T* out, RaggedParams p,
+                  uint32_t sb) {
     constexpr bool kHalf = std::is_same<T, half_t>::value;
     const uint64_t cus = uint64_t(ctx->num_cus);
     const uint64_t wide = (uint64_t(p.tokens) * p.group / kTileRows<4>) * p.kv_heads;
     const uint32_t nt = (p.head_dim + 31) / 32;
     const uint64_t slots = (nt <= 2 ? 4 : 2) * cus;  // wide tiles at once
-    p.longest_first = p.sequences <= 64 && wide >= slots && wide <= 3 * slots;
     if constexpr (kHalf) {
+        p.longest_first =
+            p.sequences <= 64 && wide >= (PAGED ? kSomeTiles : slots) && wide <= 3 * slots;
+        // Packed: eight waves of 32 rows for head size 64, 32-key blocks for 128, whose
+        // registers the mixed kernel does not leave.
+        constexpr int Q64 = PAGED ? 4 : 8;
         if (wide >= cus) {
-            if (nt == 1) launch_tiles<T, 1, 4, 1, 64, PAGED>(ctx, q, k, v, out, p);
-            else if (nt == 2) launch_tiles<T, 2, 8, 1, 64, PAGED>(ctx, q, k, v, out, p);
-            else if (nt == 3) launch_tiles<T, 3, 4, 1, 64, PAGED>(ctx, q, k, v, out, p);
-            else launch_tiles<T, 4, 4, 1, 32, PAGED>(ctx, q, k, v, out, p);
+            if (nt == 1) launch_tiles<T, 1, 4, 1, 64, PAGED>(ctx, q, k, v, out, p, sb);
+            else if (nt == 2) launch_tiles<T, 2, Q64, 1, 64, PAGED>(ctx, q, k, v, out, p, sb);
+            else if (nt == 3) launch_tiles<T, 3, 4, 1, 64, PAGED>(ctx, q, k, v, out, p, sb);
+            else launch_tiles<T, 4, 4, 1, PAGED ? 64 : 32, PAGED>(ctx, q, k, v, out, p, sb);
+        } else if (PAGED && nt == 2 && wide < kSomeTiles) {
+            launch_tiles<T, 2, 1, 4, 32, PAGED>(ctx, q, k, v, out, p, sb);
         } else {
-            if (nt == 1) launch_tiles<T, 1, 2, 2, 64, PAGED>(ctx, q, k, v, out, p);
-            else if (nt == 2) launch_tiles<T, 2, 2, 2, 64, PAGED>(ctx, q, k, v, out, p);
-            else if (nt == 3) launch_tiles<T, 3, 2, 2, 32, PAGED>(ctx, q, k, v, out, p);
-            else launch_tiles<T, 4, 2, 2, 32, PAGED>(ctx, q, k, v, out, p);
+            if (nt == 1) launch_tiles<T, 1, 2, 2, 64, PAGED>(ctx, q, k, v, out, p, sb);
+            else if (nt == 2) launch_tiles<T, 2, 2, 2, 64, PAGED>(ctx, q, k, v, out, p, sb);
+            else if (nt == 3) launch_tiles<T, 3, 2, 2, 32, PAGED>(ctx, q, k, v, out, p, sb);
+            else launch_tiles<T, 4, 2, 2, 32, PAGED>(ctx, q, k, v, out, p, sb);
         }
     } else {
         p.longest_first = p.sequences <= 64 && wide < 4 * cus;
         if (nt >= 3 && wide >= cus) {
-            if (nt == 3) launch_tiles<T, 3, 4, 1, 32, PAGED>(ctx, q, k, v, out, p);
-            else launch_tiles<T, 4, 4, 1, 32, PAGED>(ctx, q, k, v, out, p);
+            if (nt == 3) launch_tiles<T, 3, 4, 1, 32, PAGED>(ctx, q, k, v, out, p, sb);
+            else launch_tiles<T, 4, 4, 1, 32, PAGED>(ctx, q, k, v, out, p, sb);
         } else if (wide >= cus) {
-            if (nt == 1) launch_tiles<T, 1, 2, 2, 32, PAGED>(ctx, q, k, v, out, p);
-            else launch_tiles<T, 2, 2, 2, 32, PAGED>(ctx, q, k, v, out, p);
+            if (nt == 1) launch_tiles<T, 1, 2, 2, 32, PAGED>(ctx, q, k, v, out, p, sb);
+            else launch_tiles<T, 2, 2, 2, 32, PAGED>(ctx, q, k, v, out, p, sb);
         } else {
-            if (nt == 1) launch_tiles<T, 1, 1, 4, 32, PAGED>(ctx, q, k, v, out, p);
-            else if (nt == 2) launch_tiles<T, 2, 1, 4, 32, PAGED>(ctx, q, k, v, out, p);
-            else if (nt == 3) launch_tiles<T, 3, 1, 4, 32, PAGED>(ctx, q, k, v, out, p);
-            else launch_tiles<T, 4, 1, 4, 32, PAGED>(ctx, q, k, v, out, p);
+            if (nt == 1) launch_tiles<T, 1, 1, 4, 32, PAGED>(ctx, q, k, v, out, p, sb);
+            else if (nt == 2) launch_tiles<T, 2, 1, 4, 32, PAGED>(ctx, q, k, v, out, p, sb);
+            else if (nt == 3) launch_tiles<T, 3, 1, 4, 32, PAGED>(ctx, q, k, v, out, p, sb);
+            else launch_tiles<T, 4, 1, 4, 32, PAGED>(ctx, q, k, v, out, p, sb);
         }
     }
 }
@@ -1660,7 +1757,7 @@ rl_status packed_entry(rl_context* ctx, const char* name, const rl_buffer* q,
         matrix = matrix && strides[0] * es % 16 == 0 && strides[1] * es % 16 == 0 &&
                  strides[0] <= UINT32_MAX / es;
     if (matrix)
-        launch_tiles<T, false>(ctx, qd, kd, vd, od, p);
+        launch_tiles<T, false>(ctx, qd, kd, vd, od, p, 0);
     else
         launch_rows<T, false>(ctx, qd, kd, vd, od, p);
     return after_launch(ctx, name);
@@ -1750,6 +1847,7 @@ rl_status paged_entry(rl_context* ctx, const char* name, const rl_buffer* q,
                         page_bytes <= UINT32_MAX && aligned_to(qd, 16) && aligned_to(kd, 16) &&
                         aligned_to(vd, 16) && aligned_to(od, 16);
     const uint64_t most_rows = std::min(max_queries, tokens) * p.group;
+    uint32_t split_blocks = 0;
     p.page_bytes = uint32_t(page_bytes);
     p.head_bytes = uint32_t(page_size * head_dim * es);
     if (matrix && p.group <= kSplitRows) {
@@ -1759,11 +1857,16 @@ rl_status paged_entry(rl_context* ctx, const char* name, const rl_buffer* q,
         p.tickets = reinterpret_cast<uint32_t*>(ws);
         p.part = reinterpret_cast<float*>(ws + held->second.ticket_bytes);
         p.part_ml = p.part + 2 * w.slots * kv_heads * kSplitRows * 128;
-        launch_split<T>(ctx, qd, kd, vd, od, p);
-        if (most_rows <= kSplitRows) return after_launch(ctx, name);
+        if (most_rows <= kSplitRows) {
+            launch_split<T>(ctx, qd, kd, vd, od, p);
+            return after_launch(ctx, name);
+        }
+        // beside tiles: half of the workgroups that would fill the CUs
+        p.slots = uint32_t(std::max<uint64_t>(w.slots / 2, 1));
+        split_blocks = p.slots * p.kv_heads;
     }
     if (matrix)
-        launch_tiles<T, true>(ctx, qd, kd, vd, od, p);
+        launch_tiles<T, true>(ctx, qd, kd, vd, od, p, split_blocks);
     else
         launch_rows<T, true>(ctx, qd, kd, vd, od, p);
     return after_launch(ctx, name);
