@@ -173,19 +173,17 @@ SIGNATURES: dict[str, tuple[list, object]] = {
     "rl_gqa_qk_matmul_f16": ([_P, _BUF, _BUF] + [_U64] * 7 + [_BUF], _I32),
     "rl_gqa_pv_matmul_f32": ([_P, _BUF, _BUF] + [_U64] * 7 + [_BUF], _I32),
     "rl_gqa_pv_matmul_f16": ([_P, _BUF, _BUF] + [_U64] * 7 + [_BUF], _I32),
-    "rl_paged_plan": ([_P, _BUF, _BUF, _U64, _BUF, _BUF, _U64, _U64, _U64, _BUF, _BUF, _U64, _BUF,
-                       _BUF, _BUF], _I32),
-    "rl_qkv_rope_paged_append_f32": ([_P] + [_BUF, _U64P, _U64P] * 3 + [_BUF, _BUF, _U64]
-                                     + [_BUF] * 5 + [_U64] * 2, _I32),
-    "rl_qkv_rope_paged_append_f16": ([_P] + [_BUF, _U64P, _U64P] * 3 + [_BUF, _BUF, _U64]
-                                     + [_BUF] * 5 + [_U64] * 2, _I32),
-    "rl_paged_attention_workspace": ([_P] + [_U64] * 5 + [_BUF], _I32),
-    "rl_paged_attention_f32": ([_P] + [_BUF] * 6 + [_U64] * 10 + [_F, _BUF, _BUF], _I32),
-    "rl_paged_attention_f16": ([_P] + [_BUF] * 6 + [_U64] * 10 + [_F, _BUF, _BUF], _I32),
-    "rl_packed_attention_f32": ([_P] + [_BUF, _U64P, _U64P] * 3 + [_BUF, _U64, _U64, _F, _BUF],
-                                _I32),
-    "rl_packed_attention_f16": ([_P] + [_BUF, _U64P, _U64P] * 3 + [_BUF, _U64, _U64, _F, _BUF],
-                                _I32),
+    # every pointer of these as an address (DeviceBuffer.address): calls of up to
+    # 20 pointers, for which ctypes takes half the time it does for objects
+    "rl_paged_plan": ([_P] * 3 + [_U64] + [_P] * 2 + [_U64] * 3 + [_P] * 2 + [_U64] + [_P] * 3,
+                      _I32),
+    "rl_qkv_rope_paged_append_f32": ([_P] * 12 + [_U64] + [_P] * 5 + [_U64] * 2, _I32),
+    "rl_qkv_rope_paged_append_f16": ([_P] * 12 + [_U64] + [_P] * 5 + [_U64] * 2, _I32),
+    "rl_paged_attention_workspace": ([_P] + [_U64] * 5 + [_P], _I32),
+    "rl_paged_attention_f32": ([_P] * 7 + [_U64] * 10 + [_F, _P, _P], _I32),
+    "rl_paged_attention_f16": ([_P] * 7 + [_U64] * 10 + [_F, _P, _P], _I32),
+    "rl_packed_attention_f32": ([_P] * 11 + [_U64, _U64, _F, _P], _I32),
+    "rl_packed_attention_f16": ([_P] * 11 + [_U64, _U64, _F, _P], _I32),
 }
 
 # A table entry without a page, a token without a slot.
@@ -255,6 +253,21 @@ def _u64_array(values: Sequence[int]):
     return _u64_array_of(tuple(values))
 
 
+@functools.lru_cache(maxsize=256)
+def _u64_arrays_of(*values: tuple):
+    arrays = [_u64_array(v) for v in values]
+    return arrays, tuple(ctypes.addressof(a) for a in arrays)
+
+
+def _view_addresses(*views):
+    """The dims and strides of (buffer, dims, strides) views as C arrays: the
+    arrays (to be held over the call) and their addresses."""
+    shapes = []
+    for _, dims, strides in views:
+        shapes += (tuple(dims), tuple(strides))
+    return _u64_arrays_of(*shapes)
+
+
 # (op, is f16) -> the library's function, so that no name is built and looked
 # up per call.
 _FUNCTIONS: dict = {}
@@ -288,6 +301,7 @@ class DeviceBuffer:
     def raw(self, raw: RlBuffer) -> None:
         self._raw = raw
         self._as_parameter_ = ctypes.byref(raw)  # what ctypes passes for a DeviceBuffer
+        self.address = ctypes.addressof(raw)  # of the rl_buffer
 
     @property
     def len(self) -> int:
@@ -639,9 +653,10 @@ class Context:
             slots = self.empty((tokens if positions is None else positions.len,), np.uint32)
         positions = positions or self.empty((slots.len,), np.uint32)
         taken = taken or self.empty((1,), np.uint32)
-        check(self.lib.rl_paged_plan(self.handle, cached, fresh, requests, free_pages, table,
-                                     blocks, pages, page_size, offsets, context, slots.len, slots,
-                                     positions, taken))
+        check(self.lib.rl_paged_plan(self.handle, cached.address, fresh.address, requests,
+                                     free_pages.address, table.address, blocks, pages, page_size,
+                                     offsets.address, context.address, slots.len, slots.address,
+                                     positions.address, taken.address))
         return offsets, context, slots, positions, taken
 
     def qkv_rope_paged_append(self, q, k, v, cos, sin, positions, slots, k_pages, v_pages,
@@ -649,12 +664,13 @@ class Context:
         """q/k/v: (buffer, dims, strides) of [tokens, heads, D] views.  Returns
         the rotated contiguous Q; K (rotated) and V land in their slots of the
         [pages, KVH, page_size, D] pools."""
-        (qb, qd, qs), (kb, kd, ks), (vb, vd, vs) = q, k, v
-        q_out = q_out or self.empty(qd, qb.dtype)
-        self._call("qkv_rope_paged_append", qb, qb, _u64_array(qd), _u64_array(qs), kb,
-                   _u64_array(kd), _u64_array(ks), vb, _u64_array(vd), _u64_array(vs), cos, sin,
-                   cos.shape[0], positions, slots, q_out, k_pages, v_pages, k_pages.shape[0],
-                   k_pages.shape[2])
+        qb, kb, vb = q[0], k[0], v[0]
+        q_out = q_out or self.empty(q[1], qb.dtype)
+        held, (qd, qs, kd, ks, vd, vs) = _view_addresses(q, k, v)
+        self._call("qkv_rope_paged_append", qb, qb.address, qd, qs, kb.address, kd, ks, vb.address,
+                   vd, vs, cos.address, sin.address, cos.shape[0], positions.address,
+                   slots.address, q_out.address, k_pages.address, v_pages.address,
+                   k_pages.shape[0], k_pages.shape[2])
         return q_out
 
     def paged_workspace(self, sequences: int, tokens: int, q_heads: int, kv_heads: int,
@@ -680,17 +696,18 @@ class Context:
             workspace = self._workspaces.get(sizes)
             if workspace is None:
                 workspace = self._workspaces[sizes] = self.paged_workspace(*sizes)
-        self._call("paged_attention", q, q, k_pages, v_pages, table, offsets, context, requests,
-                   tokens, qh, kvh, hd, pages, page_size, blocks, max_queries, max_context, scale,
-                   workspace, out)
+        self._call("paged_attention", q, q.address, k_pages.address, v_pages.address,
+                   table.address, offsets.address, context.address, requests, tokens, qh, kvh, hd,
+                   pages, page_size, blocks, max_queries, max_context, scale, workspace.address,
+                   out.address)
         return out
 
     def packed_attention(self, q, k, v, offsets, scale: float, max_queries: int, out=None):
         """Causal attention within each packed prompt; q/k/v: (buffer, dims,
         strides) of [tokens, heads, D] views."""
-        (qb, qd, qs), (kb, kd, ks), (vb, vd, vs) = q, k, v
-        out = out or self.empty(qd, qb.dtype)
-        self._call("packed_attention", qb, qb, _u64_array(qd), _u64_array(qs), kb,
-                   _u64_array(kd), _u64_array(ks), vb, _u64_array(vd), _u64_array(vs), offsets,
-                   offsets.len - 1, max_queries, scale, out)
+        qb, kb, vb = q[0], k[0], v[0]
+        out = out or self.empty(q[1], qb.dtype)
+        held, (qd, qs, kd, ks, vd, vs) = _view_addresses(q, k, v)
+        self._call("packed_attention", qb, qb.address, qd, qs, kb.address, kd, ks, vb.address, vd,
+                   vs, offsets.address, offsets.len - 1, max_queries, scale, out.address)
         return out

@@ -83,6 +83,17 @@ __device__ inline Request load_request(const RaggedParams& p, uint32_t i) {
     return r;
 }
 
+// Lane `at`'s request in every lane.
+__device__ inline Request request_of_lane(const Request& mine, int at) {
+    Request r;
+    r.begin = uint32_t(__builtin_amdgcn_readlane(int(mine.begin), at));
+    r.n = uint32_t(__builtin_amdgcn_readlane(int(mine.n), at));
+    r.keys = uint32_t(__builtin_amdgcn_readlane(int(mine.keys), at));
+    r.bad = __builtin_amdgcn_readlane(int(mine.bad), at) != 0;
+    r.first = int64_t(r.keys) - r.n;
+    return r;
+}
+
 // The request that owns row t: the last one whose first row is not past it.
 __device__ inline uint32_t find_request(const RaggedParams& p, uint32_t t) {
     uint32_t lo = 0, hi = p.sequences;  // offsets[lo] <= t < offsets[hi], as far as they ascend
@@ -415,11 +426,7 @@ __device__ inline void split_rows(const T* __restrict__ q, const T* __restrict__
             request = base + in;
             units = uint32_t(__builtin_amdgcn_readlane(int(mine), in));
             first += uint32_t(__builtin_amdgcn_readlane(int(upto), in)) - units;
-            r.begin = uint32_t(__builtin_amdgcn_readlane(int(other.begin), in));
-            r.n = uint32_t(__builtin_amdgcn_readlane(int(other.n), in));
-            r.keys = uint32_t(__builtin_amdgcn_readlane(int(other.keys), in));
-            r.bad = __builtin_amdgcn_readlane(int(other.bad), in) != 0;
-            r.first = int64_t(r.keys) - r.n;
+            r = request_of_lane(other, in);
             break;
         }
         first += last_lane(upto);
@@ -823,14 +830,12 @@ constexpr int kTileWaves =
 
 // Up to 64 requests: tile u in the order of the keys that tiles see, most
 // first (in steps of a tile's tokens), so that the long ones do not start last.
-// Lane i counts request i's tiles at or past a level; the tile's level is the
+// Lane i, with request i in `r`, counts its tiles at or past a level; the tile's level is the
 // largest that u + 1 tiles reach.  Returns the request, its tile in `tile`;
 // `sequences` if there are not that many tiles.
-template <bool PAGED>
-__device__ inline uint32_t find_longest_tile(const RaggedParams& p, uint32_t u, uint32_t rows,
-                                             uint32_t& tile) {
+__device__ inline uint32_t find_longest_tile(const RaggedParams& p, const Request& r, uint32_t u,
+                                             uint32_t rows, uint32_t& tile) {
     const uint32_t lane = threadIdx.x % 64;
-    const Request r = load_request<PAGED>(p, min(lane, p.sequences - 1));
     const bool mine = lane < p.sequences && r.n * p.group > p.small_rows;
     const uint32_t tiles = mine ? (r.n * p.group + rows - 1) / rows : 0u;
     const uint32_t low = r.first <= 0 ? 0u : uint32_t(uint64_t(r.first) * p.group / rows);
@@ -865,18 +870,29 @@ __device__ inline bool find_tile(const RaggedParams& p, uint32_t block, uint32_t
                                  uint32_t tile_rows, uint32_t& request, Request& r,
                                  uint32_t& row0) {
     const uint32_t unit = block / p.kv_heads;
+    const uint32_t back = blocks / p.kv_heads - 1 - unit;
     uint32_t tile;
-    if (p.longest_first) {
-        request = find_longest_tile<PAGED>(p, unit, tile_rows, tile);
-        if (request >= p.sequences) return false;
+    if (p.sequences <= 64) {  // a request a lane: the lengths are read once
+        const uint32_t lane = threadIdx.x % 64;
+        const Request mine = load_request<PAGED>(p, min(lane, p.sequences - 1));
+        if (p.longest_first) {
+            request = find_longest_tile(p, mine, unit, tile_rows, tile);
+            if (request >= p.sequences) return false;
+        } else {
+            const uint32_t first = uint32_t(uint64_t(mine.begin) * p.group / tile_rows) + lane;
+            const uint64_t found = __ballot(lane < p.sequences && first <= back);
+            if (found == 0) return false;
+            request = 63u - uint32_t(__builtin_clzll(found));
+            tile = back - uint32_t(__builtin_amdgcn_readlane(int(first), int(request)));
+        }
+        r = request_of_lane(mine, int(request));
     } else {
-        const uint32_t back = blocks / p.kv_heads - 1 - unit;
         request = find_tile_request(p, back, tile_rows);
         const uint32_t first = tiles_before(p, request, tile_rows);
         if (back < first) return false;
         tile = back - first;
+        r = load_request<PAGED>(p, request);
     }
-    r = load_request<PAGED>(p, request);
     row0 = tile * tile_rows;
     const uint32_t rows = r.n * p.group;
     return uint64_t(tile) * tile_rows < rows && rows > p.small_rows;
