@@ -164,9 +164,11 @@ __global__ __launch_bounds__(kPlanThreads) void k_paged_plan(
 // (a cos - b sin, b cos + a sin) for Q into q_out and for K into row s of its
 // pages, V copied to row s; each product and sum rounded by itself, as
 // rl_rope_* does.  A thread holds N pairs' cos and sin (f32, 2 N values) and
-// turns them for `kHeads` heads of its token, so that the tables cost
-// 8 / kHeads of the bytes of an f16 row instead of 2 times them.  Lanes run
-// along a row, then over heads: whole rows on consecutive lanes.
+// turns them for `kHeads` heads of its token, so that the tables (L2) cost
+// 2 / kHeads times the bytes of an f16 row.  Lanes run along a row, then over
+// heads: whole rows on consecutive lanes.  Bound by HBM: 35.2 us for 8223 tokens
+// of 32/8 heads of 128 in f16 (206 MB, 5.9 TB/s; a plain copy of as much runs at
+// 4.9), by its launch below some hundred tokens.
 struct RowsView {
     uint64_t token_stride;
     uint64_t head_stride;
@@ -185,7 +187,7 @@ struct AppendParams {
     uint64_t slots;  // of the whole pool
 };
 
-template <typename T, int N, int kHeads>
+template <typename T, int N, int kHeads, bool STREAM_IN, bool STREAM_OUT>
 __global__ __launch_bounds__(256) void k_paged_append(
     const T* __restrict__ q, const T* __restrict__ k, const T* __restrict__ v,
     const float* __restrict__ cos_table, const float* __restrict__ sin_table,
@@ -213,8 +215,10 @@ __global__ __launch_bounds__(256) void k_paged_append(
             : head < rotated
                 ? k + token * p.k.token_stride + (head - p.q_heads) * p.k.head_stride
                 : v + token * p.v.token_stride + (head - rotated) * p.v.head_stride;
-        a[j] = *reinterpret_cast<const V*>(src + pair);
-        b[j] = *reinterpret_cast<const V*>(src + p.half_dim + pair);
+        const V* first = reinterpret_cast<const V*>(src + pair);
+        const V* second = reinterpret_cast<const V*>(src + p.half_dim + pair);
+        a[j] = STREAM_IN ? load_stream(first) : *first;
+        b[j] = STREAM_IN ? load_stream(second) : *second;
     }
     const uint32_t position = positions[token], slot = slots[token];
     if (slot >= p.slots || position >= p.table_rows) return;
@@ -244,8 +248,15 @@ __global__ __launch_bounds__(256) void k_paged_append(
                 y[e] = from_float<T>(second * c[e] + first * s[e]);
             }
         }
-        *reinterpret_cast<V*>(dst + pair) = x;
-        *reinterpret_cast<V*>(dst + p.half_dim + pair) = y;
+        V* first = reinterpret_cast<V*>(dst + pair);
+        V* second = reinterpret_cast<V*>(dst + p.half_dim + pair);
+        if constexpr (STREAM_OUT) {
+            store_stream(first, x);
+            store_stream(second, y);
+        } else {
+            *first = x;
+            *second = y;
+        }
     }
 }
 
@@ -368,6 +379,8 @@ rl_status plan_entry(rl_context* ctx, const rl_buffer* cached, const rl_buffer* 
     return after_launch(ctx, "paged_plan");
 }
 
+constexpr uint64_t kStreamRows = uint64_t(88) << 20;
+
 template <typename T, int N>
 void launch_append(rl_context* ctx, uint64_t tokens, uint64_t heads, AppendParams p, const T* q,
                    const T* k, const T* v, const float* cos_table, const float* sin_table,
@@ -375,17 +388,25 @@ void launch_append(rl_context* ctx, uint64_t tokens, uint64_t heads, AppendParam
                    T* v_pages) {
     const uint64_t packs = p.half_dim / N;
     p.packs = FastDiv(uint32_t(packs));
+    // Few items: a thread a head, so that there are enough of them.  Many: four
+    // heads a thread and streamed stores; from kStreamRows of rows on, more than the
+    // MALL keeps beside what is written, streamed loads too, with two heads a thread
+    // (one MI355X, 32/8 heads of 128 in f16: 2079 tokens, 26 MB of rows, 9.6 us with
+    // plain loads, 10.7 streamed, 10.3 with plain stores as well; 5663, 70 MB, 21.9 /
+    // 25.2; 8223, 101 MB, 37.2 / 35.2, 44.3).
     const bool many = tokens * heads * packs >= uint64_t(ctx->num_cus) * 2048;
-    const uint64_t steps = many ? ceil_div(heads, 4) : heads;
+    const bool stream = many && tokens * heads * 2 * p.half_dim * sizeof(T) >= kStreamRows;
+    const uint64_t steps = ceil_div(heads, stream ? 2 : many ? 4 : 1);
     p.head_steps = FastDiv(uint32_t(steps));
     p.items = uint32_t(tokens * steps * packs);
     const dim3 grid(unsigned(ceil_div(p.items, 256))), block(256);
-    if (many)
-        RL_LAUNCH(ctx, (k_paged_append<T, N, 4>), grid, block, q, k, v, cos_table, sin_table,
-                  positions, slots, q_out, k_pages, v_pages, p);
-    else
-        RL_LAUNCH(ctx, (k_paged_append<T, N, 1>), grid, block, q, k, v, cos_table, sin_table,
-                  positions, slots, q_out, k_pages, v_pages, p);
+#define RL_APPEND(HEADS, IN, OUT)                                                             \
+    RL_LAUNCH(ctx, (k_paged_append<T, N, HEADS, IN, OUT>), grid, block, q, k, v, cos_table,   \
+              sin_table, positions, slots, q_out, k_pages, v_pages, p)
+    if (stream) RL_APPEND(2, true, true);
+    else if (many) RL_APPEND(4, false, true);
+    else RL_APPEND(1, false, false);
+#undef RL_APPEND
 }
 
 template <typename T>
