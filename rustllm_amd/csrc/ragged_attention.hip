@@ -1629,9 +1629,14 @@ rl_status check_batch(uint64_t sequences, uint64_t tokens, uint64_t q_heads, uin
     if (kv_heads == 0 || q_heads % kv_heads != 0)
         return fail(RL_ERR_MODEL_FORMAT, "Q heads %llu must be divisible by non-zero KV heads %llu",
                     (unsigned long long)q_heads, (unsigned long long)kv_heads);
-    if (sequences >= UINT32_MAX || tokens > UINT32_MAX || q_heads > UINT32_MAX ||
-        max_queries > UINT32_MAX || tokens > UINT32_MAX / q_heads)
+    // positions and key counts are signed 32-bit numbers in the kernels, and a
+    // launch has fewer than 2^32 threads
+    if (sequences > INT32_MAX || tokens > INT32_MAX || max_queries > UINT32_MAX ||
+        q_heads > UINT32_MAX || tokens > UINT32_MAX / q_heads)
         return fail(RL_ERR_INVALID_SHAPE, "attention row count exceeds u32");
+    if (sequences * kv_heads >= (uint64_t(1) << 23))
+        return fail(RL_ERR_INVALID_SHAPE, "%llu requests of %llu KV heads exceed one launch",
+                    (unsigned long long)sequences, (unsigned long long)kv_heads);
     if (head_dim > 512)
         return fail(RL_ERR_INVALID_SHAPE, "attention head size %llu exceeds 512",
                     (unsigned long long)head_dim);
@@ -1642,8 +1647,13 @@ rl_status check_batch(uint64_t sequences, uint64_t tokens, uint64_t q_heads, uin
 }
 
 template <typename T, bool PAGED>
-void launch_rows(rl_context* ctx, const T* q, const T* k, const T* v, T* out,
-                 const RaggedParams& p) {
+rl_status launch_rows(rl_context* ctx, const char* name, const T* q, const T* k, const T* v,
+                      T* out, const RaggedParams& p) {
+    if (uint64_t(p.tokens) * p.q_heads >= (uint64_t(1) << 26))
+        return fail(RL_ERR_INVALID_SHAPE,
+                    "%u rows of %u heads exceed one launch (head size, strides or alignment off "
+                    "the matrix-core kernels')",
+                    p.tokens, p.q_heads);
     const dim3 grid(p.tokens * p.q_heads), block(64);
     if (p.head_dim <= 64)
         RL_LAUNCH(ctx, (k_ragged_rows<T, 1, PAGED>), grid, block, q, k, v, out, p);
@@ -1653,6 +1663,7 @@ void launch_rows(rl_context* ctx, const T* q, const T* k, const T* v, T* out,
         RL_LAUNCH(ctx, (k_ragged_rows<T, 4, PAGED>), grid, block, q, k, v, out, p);
     else
         RL_LAUNCH(ctx, (k_ragged_rows<T, 8, PAGED>), grid, block, q, k, v, out, p);
+    return after_launch(ctx, name);
 }
 
 // The tile kernels for a batch of at most `tokens` rows; paged ones with
@@ -1790,10 +1801,8 @@ rl_status packed_entry(rl_context* ctx, const char* name, const rl_buffer* q,
     for (const uint64_t* strides : {q_strides, k_strides, v_strides})
         matrix = matrix && strides[0] * es % 16 == 0 && strides[1] * es % 16 == 0 &&
                  strides[0] <= UINT32_MAX / es;
-    if (matrix)
-        launch_tiles<T, false>(ctx, qd, kd, vd, od, p, 0);
-    else
-        launch_rows<T, false>(ctx, qd, kd, vd, od, p);
+    if (!matrix) return launch_rows<T, false>(ctx, name, qd, kd, vd, od, p);
+    launch_tiles<T, false>(ctx, qd, kd, vd, od, p, 0);
     return after_launch(ctx, name);
 }
 
@@ -1812,8 +1821,8 @@ rl_status paged_entry(rl_context* ctx, const char* name, const rl_buffer* q,
     if (rl_status st = check_pages(pages, page_size)) return st;
     if (max_blocks == 0 || max_context == 0)
         return fail(RL_ERR_INVALID_SHAPE, "attention dimensions must be greater than zero");
-    if (max_blocks > UINT32_MAX || max_context >= UINT32_MAX)
-        return fail(RL_ERR_INVALID_SHAPE, "attention key range exceeds u32");
+    if (max_blocks > UINT32_MAX || max_context > INT32_MAX)
+        return fail(RL_ERR_INVALID_SHAPE, "attention key range exceeds i32");
     if (max_context > max_blocks * page_size)
         return fail(RL_ERR_INVALID_SHAPE,
                     "a context of %llu exceeds a table row of %llu pages of %llu positions",
@@ -1899,10 +1908,8 @@ rl_status paged_entry(rl_context* ctx, const char* name, const rl_buffer* q,
         p.slots = uint32_t(std::max<uint64_t>(w.slots / 2, 1));
         split_blocks = p.slots * p.kv_heads;
     }
-    if (matrix)
-        launch_tiles<T, true>(ctx, qd, kd, vd, od, p, split_blocks);
-    else
-        launch_rows<T, true>(ctx, qd, kd, vd, od, p);
+    if (!matrix) return launch_rows<T, true>(ctx, name, qd, kd, vd, od, p);
+    launch_tiles<T, true>(ctx, qd, kd, vd, od, p, split_blocks);
     return after_launch(ctx, name);
 }
 

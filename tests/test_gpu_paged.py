@@ -309,6 +309,12 @@ PAGED = [
     ([(3, 2), (300, 1)], 2, 2, 512, 16),
     ([(2900, 600), (5, 1)], 8, 2, 64, 64),          # few tiles over many keys
     ([(3500, 130)], 4, 1, 128, 32),
+    # enough rows for the wide tiles, and for ordering them by length
+    ([(100, 300), (0, 310), (700, 290), (5, 1), (33, 300)], 32, 8, 64, 16),
+    ([(100, 300), (0, 310), (5, 2), (300, 450)], 32, 8, 128, 32),
+    ([(70, 500), (0, 310), (5, 1), (300, 300)], 32, 8, 96, 16),
+    ([(70, 500), (0, 310), (5, 3), (300, 300)], 32, 8, 32, 64),
+    ([(40, 200), (0, 310), (5, 1), (1300, 290)], 15, 5, 64, 16),
 ]
 
 
@@ -481,6 +487,38 @@ def test_recorded_attention_follows_its_lengths(ctx, dtype, spans):
         ctx.graph_destroy(graph)
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("n", [1, 40])
+def test_pools_past_4_gib(ctx, dtype, n):
+    """Pages whose bytes and elements lie past 2^32 (32 GiB of pool in all, of which a few
+    pages are written and read)."""
+    qh, kvh, d, page = 4, 2, 128, 64
+    pages = 9 * (1 << 30) // (kvh * page * d)  # 9 Gi elements a pool
+    spans = [(150, n), (70, n)]
+    b = Batch(spans, qh, kvh, d, page, dtype, ("far", n))
+    far = {int(p): pages - 1 - 100 * i for i, p in enumerate(b.table[b.table != NONE])}
+    dk, dv = (ctx.empty((pages, kvh, page, d), dtype) for _ in range(2))
+    tokens = int(b.context.sum())
+    slots = np.concatenate([[far[int(b.table[i, p // page])] * page + p % page
+                             for p in range(c + m)] for i, (c, m) in enumerate(spans)])
+    ones, zeros = np.ones((1, d // 2), np.float32), np.zeros((1, d // 2), np.float32)
+    k, v = np.concatenate(b.k), np.concatenate(b.v)
+    q = np.zeros((tokens, qh, d), dtype)
+    view = lambda x: (ctx.upload(x), x.shape, (x.shape[1] * d, d, 1))
+    ctx.qkv_rope_paged_append(view(q), view(k), view(v), ctx.upload(ones), ctx.upload(zeros),
+                              ctx.upload(np.zeros(tokens, np.uint32)),
+                              ctx.upload(slots.astype(np.uint32)), dk, dv)
+    table = np.array([[far.get(int(p), NONE) for p in row] for row in b.table], np.uint32)
+    out = ctx.upload(np.full(b.q.shape, 7.0, dtype))
+    ctx.paged_attention(ctx.upload(b.q), dk, dv, ctx.upload(table), ctx.upload(b.offsets),
+                        ctx.upload(b.context), b.scale, b.max_queries, b.max_context, out)
+    ctx.finish()
+    b.check(out.numpy())
+    dk.release()
+    dv.release()
+    abi.check(ctx.lib.rl_context_trim(ctx.handle))
+
+
 def test_two_contexts_serve_their_own_batches(ctx):
     """Calls of two contexts (streams) at once, each with its own workspace."""
     other = abi.Context(0)
@@ -594,6 +632,10 @@ PACKED = [
     ([100, 50], 6, 3, 32), ([19, 40], 4, 2, 48), ([9, 6], 2, 1, 7), ([5, 9], 2, 2, 200),
     ([3, 8], 1, 1, 512), ([700, 600], 16, 1, 64), ([60, 90], 40, 1, 64), ([1500], 9, 3, 64),
     ([1100, 900, 3], 8, 8, 128), ([2, 3] * 100, 6, 2, 64),
+    # enough rows for the wide tiles (and, the last, to order them by length)
+    ([700, 500, 33, 64], 32, 8, 64), ([600, 511, 1], 32, 8, 128), ([400, 700], 32, 8, 96),
+    ([900, 300], 32, 8, 32), ([260, 30, 511] * 6, 32, 8, 64), ([130, 300] * 10, 32, 8, 128),
+    ([40] * 80 + [900], 32, 8, 64),
 ]
 
 

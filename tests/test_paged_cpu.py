@@ -129,6 +129,10 @@ def test_paged_attention_validation(dt, es):
     assert st == SHAPE and "row count exceeds u32" in msg
     st, msg = go(pages=1 << 29, page=16)
     assert st == SHAPE and "u32 slots" in msg
+    st, msg = go(s=1 << 22, kvh=2)
+    assert st == SHAPE and "exceed one launch" in msg
+    st, msg = go(mc=1 << 31, blocks=1 << 28)
+    assert st == SHAPE and "key range exceeds" in msg
     assert go(page=20)[0] == SHAPE
     for name in ("q", "kp", "vp", "out"):
         assert go(**{name: buf(7, es)})[0] == SHAPE, name
