@@ -596,12 +596,14 @@ rl_status rl_qkv_rope_paged_append_f16(
     const rl_buffer* positions, const rl_buffer* slots, const rl_buffer* q_out,
     const rl_buffer* k_pages, const rl_buffer* v_pages, uint64_t pages, uint64_t page_size);
 
-/* Memory for rl_paged_attention_* calls of up to these sizes (release it with
- * rl_buffer_release).  It serves one call at a time: calls that may overlap
- * (contexts on other streams) need one each; calls in order on one context,
- * and graphs replayed on it, can share one.  Not while recording. */
-rl_status rl_paged_attention_workspace(rl_context* ctx, uint64_t sequences, uint64_t tokens,
-                                       uint64_t q_heads, uint64_t kv_heads, uint64_t head_dim,
+/* Memory for rl_paged_attention_* calls of up to `sequences` requests and
+ * `kv_heads` KV heads: the partial results and hand-over counters of requests
+ * whose keys several workgroups share.  Release it with rl_buffer_release.  It
+ * serves one call at a time: calls that may overlap (contexts on other
+ * streams, a graph replayed on another context) need one each; calls in order
+ * on one context, and graphs replayed on it, can share one.  Not while
+ * recording. */
+rl_status rl_paged_attention_workspace(rl_context* ctx, uint64_t sequences, uint64_t kv_heads,
                                        rl_buffer* out);
 /* rl_attention_* of every request's new tokens over its pages, single tokens
  * and chunks in one call: row offsets[i] + j is request i's position

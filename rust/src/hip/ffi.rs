@@ -736,10 +736,7 @@ extern "C" {
     pub fn rl_paged_attention_workspace(
         ctx: *mut rl_context,
         sequences: u64,
-        tokens: u64,
-        q_heads: u64,
         kv_heads: u64,
-        head_dim: u64,
         out: *mut rl_buffer,
     ) -> rl_status;
     pub fn rl_paged_attention_f32(

@@ -179,7 +179,7 @@ SIGNATURES: dict[str, tuple[list, object]] = {
                       _I32),
     "rl_qkv_rope_paged_append_f32": ([_P] * 12 + [_U64] + [_P] * 5 + [_U64] * 2, _I32),
     "rl_qkv_rope_paged_append_f16": ([_P] * 12 + [_U64] + [_P] * 5 + [_U64] * 2, _I32),
-    "rl_paged_attention_workspace": ([_P] + [_U64] * 5 + [_P], _I32),
+    "rl_paged_attention_workspace": ([_P, _U64, _U64, _P], _I32),
     "rl_paged_attention_f32": ([_P] * 7 + [_U64] * 10 + [_F, _P, _P], _I32),
     "rl_paged_attention_f16": ([_P] * 7 + [_U64] * 10 + [_F, _P, _P], _I32),
     "rl_packed_attention_f32": ([_P] * 11 + [_U64, _U64, _F, _P], _I32),
@@ -673,12 +673,11 @@ class Context:
                    k_pages.shape[0], k_pages.shape[2])
         return q_out
 
-    def paged_workspace(self, sequences: int, tokens: int, q_heads: int, kv_heads: int,
-                        head_dim: int) -> DeviceBuffer:
+    def paged_workspace(self, sequences: int, kv_heads: int) -> DeviceBuffer:
         """Memory for paged_attention() calls of up to these sizes, one at a time."""
         raw = RlBuffer()
-        check(self.lib.rl_paged_attention_workspace(self.handle, sequences, tokens, q_heads,
-                                                    kv_heads, head_dim, ctypes.byref(raw)))
+        check(self.lib.rl_paged_attention_workspace(self.handle, sequences, kv_heads,
+                                                    ctypes.byref(raw)))
         return DeviceBuffer(self, raw, np.uint8, (raw.len,))
 
     def paged_attention(self, q, k_pages, v_pages, table, offsets, context, scale: float,
@@ -686,13 +685,13 @@ class Context:
         """Attention of each request's rows of q [tokens, QH, D] over its pages
         of the [pages, KVH, page_size, D] pools.  Without a `workspace` the
         context makes and keeps its own, one for each power of two of requests
-        and rows (so a step to be recorded runs once before)."""
+        and KV heads (so a step to be recorded runs once before)."""
         tokens, qh, hd = q.shape
         pages, kvh, page_size, _ = k_pages.shape
         requests, blocks = table.shape
         out = out or self.empty(q.shape, q.dtype)
         if workspace is None:
-            sizes = (_power_of_two(requests), _power_of_two(tokens), qh, kvh, hd)
+            sizes = (_power_of_two(requests), _power_of_two(kvh))
             workspace = self._workspaces.get(sizes)
             if workspace is None:
                 workspace = self._workspaces[sizes] = self.paged_workspace(*sizes)

@@ -66,7 +66,7 @@ struct Request {
     uint32_t begin;  // first row
     uint32_t n;      // rows
     uint32_t keys;
-    int64_t first;  // position of the first row
+    int32_t first;  // position of the first row
     bool bad;       // more keys than max_context
 };
 
@@ -75,11 +75,12 @@ __device__ inline Request load_request(const RaggedParams& p, uint32_t i) {
     Request r;
     r.begin = min(p.offsets[i], p.tokens);
     const uint32_t end = min(p.offsets[i + 1], p.tokens);
-    r.n = end > r.begin ? min(end - r.begin, p.max_queries) : 0u;
+    const uint32_t all = end > r.begin ? end - r.begin : 0u;
+    r.n = min(all, p.max_queries);
     const uint32_t ctx = PAGED ? p.context[i] : r.n;
     r.bad = PAGED && ctx > p.max_context;
     r.keys = PAGED ? min(ctx, p.max_context) : ctx;
-    r.first = int64_t(r.keys) - r.n;
+    r.first = PAGED ? int32_t(r.keys) - int32_t(all) : 0;
     return r;
 }
 
@@ -90,7 +91,7 @@ __device__ inline Request request_of_lane(const Request& mine, int at) {
     r.n = uint32_t(__builtin_amdgcn_readlane(int(mine.n), at));
     r.keys = uint32_t(__builtin_amdgcn_readlane(int(mine.keys), at));
     r.bad = __builtin_amdgcn_readlane(int(mine.bad), at) != 0;
-    r.first = int64_t(r.keys) - r.n;
+    r.first = __builtin_amdgcn_readlane(mine.first, at);
     return r;
 }
 
@@ -136,7 +137,7 @@ __device__ inline void row_by_wave(const T* __restrict__ q, const T* __restrict_
                                    uint32_t j, uint32_t head) {
     const uint32_t lane = threadIdx.x % 64, D = p.head_dim, kv_head = head / p.group;
     const T* qrow = q + (r.begin + j) * p.q_token + head * p.q_head;
-    const int64_t position = r.first + j;
+    const int64_t position = int64_t(r.first) + j;
     const uint32_t key_end = position < 0 ? 0u : uint32_t(position) + 1;
     float o[2] = {0.0f, 0.0f}, m = -INFINITY, l = 0.0f;
     for (uint32_t base = 0; base < key_end; base += 64) {
@@ -201,7 +202,7 @@ __global__ __launch_bounds__(64) void k_ragged_rows(const T* __restrict__ q,
     const Request r = load_request<PAGED>(p, i);
     if (t < r.begin || t - r.begin >= r.n || r.n * p.group <= p.small_rows) return;
     const uint32_t D = p.head_dim, kv_head = head / p.group;
-    const int64_t position = r.first + (t - r.begin);
+    const int64_t position = int64_t(r.first) + (t - r.begin);
     const uint32_t key_end = position < 0 ? 0u : uint32_t(position) + 1;
 #pragma unroll
     for (int e = 0; e < DT; ++e) {
@@ -512,7 +513,7 @@ __device__ inline void split_rows(const T* __restrict__ q, const T* __restrict__
     // row lr of this KV head: query elements, last key it sees (-1: none)
     const bool row_live = lr < R;
     const uint32_t token = row_live ? lr / p.group : 0u, sub = row_live ? lr % p.group : 0u;
-    const int64_t position = r.first + token;
+    const int64_t position = int64_t(r.first) + token;
     const int limit = row_live && position >= 0 ? int(min(int64_t(last), position)) : -1;
     const T* qrow = q + (r.begin + token) * p.q_token + (kvh * p.group + sub) * p.q_head;
     KV qf[S::kKChunks];
@@ -658,7 +659,7 @@ __device__ inline void split_rows(const T* __restrict__ q, const T* __restrict__
     // row `row`'s output, two elements: stored unless it is not finite
     auto store_row = [&](uint32_t row, uint32_t d, float2 x, float sum) {
         const uint32_t tok = row / p.group;
-        const int64_t pos = r.first + tok;
+        const int64_t pos = int64_t(r.first) + tok;
         const float inv = pos < 0 ? 0.0f : 1.0f / sum;
         x.x *= inv;
         x.y *= inv;
@@ -856,7 +857,10 @@ __device__ inline uint32_t find_longest_tile(const RaggedParams& p, const Reques
     const uint32_t lane = threadIdx.x % 64;
     const bool mine = lane < p.sequences && r.n * p.group > p.small_rows;
     const uint32_t tiles = mine ? (r.n * p.group + rows - 1) / rows : 0u;
-    const uint32_t low = r.first <= 0 ? 0u : uint32_t(uint64_t(r.first) * p.group / rows);
+    // (bounded, so that levels stay below 2^31)
+    const uint32_t low =
+        r.first <= 0 ? 0u
+                     : uint32_t(min(uint64_t(r.first) * p.group / rows, uint64_t(1) << 29));
     auto reach = [&](uint32_t level) {  // this request's tiles at or past it
         return min(tiles, low + tiles > level ? low + tiles - level : 0u);
     };
@@ -965,7 +969,7 @@ __device__ inline void tile_rows(const half_t* __restrict__ q, const half_t* __r
     const uint32_t last = r.keys == 0 ? 0u : r.keys - 1;
     // keys that the tile's last row sees
     auto keys_of = [&](uint32_t row) {  // visible to row `row` of the request
-        const int64_t pos = r.first + row / p.group;
+        const int64_t pos = int64_t(r.first) + row / p.group;
         return pos < 0 || r.bad ? 0u : uint32_t(min(int64_t(r.keys), pos + 1));
     };
     const uint32_t keys = keys_of(min(row0 + TILE, rows) - 1);
@@ -1278,7 +1282,7 @@ __device__ inline void tile_rows_f32(const float* __restrict__ q, const float* _
     const uint32_t col = lane % 32, hs = lane / 32;
     const uint32_t last = r.keys == 0 ? 0u : r.keys - 1;
     auto keys_of = [&](uint32_t row) {  // visible to row `row` of the request
-        const int64_t pos = r.first + row / p.group;
+        const int64_t pos = int64_t(r.first) + row / p.group;
         return pos < 0 || r.bad ? 0u : uint32_t(min(int64_t(r.keys), pos + 1));
     };
     const uint32_t wrow0 = row0 + 32 * qw;
@@ -1606,20 +1610,20 @@ __global__ __launch_bounds__(64 * QW * KS, (Tile<T, NT, QW, KS, BN>::kWaves)) vo
 //
 // The split kernel's workgroups (two fit a CU: registers), their partials and
 // tickets.
-struct WorkspaceNeed {
-    uint64_t slots;
-    rl_context::Workspace size;
-};
+uint64_t split_slots(const rl_context* ctx, uint64_t kv_heads) {  // a KV head's
+    return std::max<uint64_t>(2 * uint64_t(ctx->num_cus) / kv_heads, 1);
+}
 
-WorkspaceNeed workspace_for(const rl_context* ctx, uint64_t sequences, uint64_t kv_heads) {
-    WorkspaceNeed w{};
-    w.slots = std::max<uint64_t>(2 * uint64_t(ctx->num_cus) / kv_heads, 1);
-    w.size.ticket_bytes = sequences * kv_heads * kTicketStride * sizeof(uint32_t);
-    w.size.partial_bytes = 2 * w.slots * kv_heads * kSplitRows * (128 + 2) * sizeof(float);
-    return w;
+// What a call of these sizes needs; no less for more requests or KV heads.
+rl_context::Workspace workspace_for(const rl_context* ctx, uint64_t sequences, uint64_t kv_heads) {
+    const uint64_t groups = std::max<uint64_t>(2 * uint64_t(ctx->num_cus), kv_heads);
+    return {sequences * kv_heads * kTicketStride * sizeof(uint32_t),
+            2 * groups * kSplitRows * (128 + 2) * sizeof(float)};
 }
 
 // ------------------------------------------------------------- validation
+
+constexpr uint64_t kMostRows = uint64_t(1) << 29;
 
 // Checks shared by both attentions, the rows' part.
 rl_status check_batch(uint64_t sequences, uint64_t tokens, uint64_t q_heads, uint64_t kv_heads,
@@ -1629,11 +1633,11 @@ rl_status check_batch(uint64_t sequences, uint64_t tokens, uint64_t q_heads, uin
     if (kv_heads == 0 || q_heads % kv_heads != 0)
         return fail(RL_ERR_MODEL_FORMAT, "Q heads %llu must be divisible by non-zero KV heads %llu",
                     (unsigned long long)q_heads, (unsigned long long)kv_heads);
-    // positions and key counts are signed 32-bit numbers in the kernels, and a
-    // launch has fewer than 2^32 threads
-    if (sequences > INT32_MAX || tokens > INT32_MAX || max_queries > UINT32_MAX ||
-        q_heads > UINT32_MAX || tokens > UINT32_MAX / q_heads)
-        return fail(RL_ERR_INVALID_SHAPE, "attention row count exceeds u32");
+    // a launch has fewer than 2^32 threads, at most 256 for 64 rows of all heads
+    if (sequences > INT32_MAX || max_queries > UINT32_MAX || q_heads > kMostRows ||
+        tokens > kMostRows / q_heads)
+        return fail(RL_ERR_INVALID_SHAPE, "%llu rows of %llu heads exceed one launch",
+                    (unsigned long long)tokens, (unsigned long long)q_heads);
     if (sequences * kv_heads >= (uint64_t(1) << 23))
         return fail(RL_ERR_INVALID_SHAPE, "%llu requests of %llu KV heads exceed one launch",
                     (unsigned long long)sequences, (unsigned long long)kv_heads);
@@ -1845,19 +1849,20 @@ rl_status paged_entry(rl_context* ctx, const char* name, const rl_buffer* q,
     if (rl_status st = check_output(out, numel, es, "paged attention")) return st;
     if (rl_status st = check_buffer(workspace, "workspace")) return st;
     if (rl_status st = require_context(ctx)) return st;
-    const WorkspaceNeed w = workspace_for(ctx, sequences, kv_heads);
+    const rl_context::Workspace need = workspace_for(ctx, sequences, kv_heads);
+    const uint64_t slots = split_slots(ctx, kv_heads);
     const auto held = ctx->workspaces.find(workspace->data);
     if (held == ctx->workspaces.end())
         return fail(RL_ERR_INVALID_ARGUMENT,
                     "the workspace is not one of rl_paged_attention_workspace on this context");
-    if (held->second.ticket_bytes < w.size.ticket_bytes ||
-        held->second.partial_bytes < w.size.partial_bytes)
+    if (held->second.ticket_bytes < need.ticket_bytes ||
+        held->second.partial_bytes < need.partial_bytes)
         return fail(RL_ERR_INVALID_SHAPE,
                     "the workspace holds %llu + %llu bytes, expected %llu + %llu",
                     (unsigned long long)held->second.ticket_bytes,
                     (unsigned long long)held->second.partial_bytes,
-                    (unsigned long long)w.size.ticket_bytes,
-                    (unsigned long long)w.size.partial_bytes);
+                    (unsigned long long)need.ticket_bytes,
+                    (unsigned long long)need.partial_bytes);
     if (rl_status st = activate(ctx)) return st;
 
     RaggedParams p{};
@@ -1896,16 +1901,16 @@ rl_status paged_entry(rl_context* ctx, const char* name, const rl_buffer* q,
     if (matrix && p.group <= kSplitRows) {
         char* ws = static_cast<char*>(workspace->data);
         p.small_rows = kSplitRows;
-        p.slots = uint32_t(w.slots);
+        p.slots = uint32_t(slots);
         p.tickets = reinterpret_cast<uint32_t*>(ws);
         p.part = reinterpret_cast<float*>(ws + held->second.ticket_bytes);
-        p.part_ml = p.part + 2 * w.slots * kv_heads * kSplitRows * 128;
+        p.part_ml = p.part + 2 * slots * kv_heads * kSplitRows * 128;
         if (most_rows <= kSplitRows) {
             launch_split<T>(ctx, qd, kd, vd, od, p);
             return after_launch(ctx, name);
         }
         // beside tiles: half of the workgroups that would fill the CUs
-        p.slots = uint32_t(std::max<uint64_t>(w.slots / 2, 1));
+        p.slots = uint32_t(std::max<uint64_t>(slots / 2, 1));
         split_blocks = p.slots * p.kv_heads;
     }
     if (!matrix) return launch_rows<T, true>(ctx, name, qd, kd, vd, od, p);
@@ -1913,16 +1918,15 @@ rl_status paged_entry(rl_context* ctx, const char* name, const rl_buffer* q,
     return after_launch(ctx, name);
 }
 
-rl_status workspace_entry(rl_context* ctx, uint64_t sequences, uint64_t tokens, uint64_t q_heads,
-                          uint64_t kv_heads, uint64_t head_dim, rl_buffer* out) {
+rl_status workspace_entry(rl_context* ctx, uint64_t sequences, uint64_t kv_heads,
+                          rl_buffer* out) {
     if (out == nullptr) return fail(RL_ERR_INVALID_ARGUMENT, "output buffer pointer is null");
     *out = rl_buffer{nullptr, 0, 0};
-    if (rl_status st = check_batch(sequences, tokens, q_heads, kv_heads, head_dim, 1, 1.0f))
-        return st;
+    if (rl_status st = check_batch(sequences, 1, kv_heads, kv_heads, 1, 1, 1.0f)) return st;
     if (rl_status st = require_context(ctx)) return st;
     if (ctx->capturing)
         return fail(RL_ERR_DEVICE, "a workspace cannot be made while recording a graph");
-    const rl_context::Workspace size = workspace_for(ctx, sequences, kv_heads).size;
+    const rl_context::Workspace size = workspace_for(ctx, sequences, kv_heads);
     const uint64_t bytes = size.ticket_bytes + size.partial_bytes;
     rl_buffer made{nullptr, 0, 0};
     if (rl_status st = rl_buffer_empty(ctx, bytes, 1, &made)) return st;
@@ -1943,12 +1947,9 @@ using namespace rl;
 
 extern "C" {
 
-rl_status rl_paged_attention_workspace(rl_context* ctx, uint64_t sequences, uint64_t tokens,
-                                       uint64_t q_heads, uint64_t kv_heads, uint64_t head_dim,
+rl_status rl_paged_attention_workspace(rl_context* ctx, uint64_t sequences, uint64_t kv_heads,
                                        rl_buffer* out) {
-    return guarded([&] {
-        return workspace_entry(ctx, sequences, tokens, q_heads, kv_heads, head_dim, out);
-    });
+    return guarded([&] { return workspace_entry(ctx, sequences, kv_heads, out); });
 }
 
 rl_status rl_paged_attention_f32(rl_context* ctx, const rl_buffer* q, const rl_buffer* k_pages,

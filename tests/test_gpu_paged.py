@@ -347,6 +347,36 @@ def test_paged_attention_bounds_may_be_loose(ctx, dtype):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
+def test_rows_past_max_queries_are_left(ctx, dtype):
+    """A request of more rows than max_queries: its first ones as they are, the rest
+    not written; the same for packed prompts."""
+    for most in (2, 40):
+        b = Batch([(100, 60), (7, 1)], 6, 2, 64, 16, dtype, ("most", most))
+        got = b.run(ctx, max_queries=most)
+        _, exact, bound = b.expect(0)
+        err = np.abs(got[:most].astype(np.float64).transpose(1, 0, 2) - exact[:, :most])
+        assert np.all(err <= bound[:, :most])
+        assert np.all(got[most:60] == 7.0)
+        b.check(got, skip=(0,))
+
+
+def test_one_workspace_serves_batches_of_many_sizes(ctx):
+    """Calls of different numbers of requests and KV heads take turns with one
+    workspace (its counters are zero again after each)."""
+    workspace = ctx.paged_workspace(40, 8)
+    batches = [Batch([(900, 1)] * n, qh, kvh, 64, 16, np.float16, ("turns", n, kvh))
+               for n, qh, kvh in ((40, 8, 8), (1, 6, 2), (7, 15, 5), (40, 4, 1))]
+    held = [(b, b.upload(ctx)) for b in batches]
+    for _ in range(3):
+        for b, d in held:
+            out = ctx.upload(np.full(b.q.shape, 7.0, np.float16))
+            ctx.paged_attention(d["q"], d["kp"], d["vp"], d["table"], d["offsets"], d["context"],
+                                b.scale, 1, b.max_context, out, workspace)
+            ctx.finish()
+            b.check(out.numpy())
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("n", [1, 40])
 def test_paged_attention_marks_what_is_not_there(ctx, dtype, n):
     """Rows that see a key of a page outside the pool are NaN, so is a request
@@ -549,7 +579,7 @@ def test_the_workspace_is_this_contexts_and_large_enough(ctx):
 
     with pytest.raises(abi.RustLLMError, match="not one of rl_paged_attention_workspace"):
         go(ctx.empty((1 << 20,), np.uint8))
-    good = ctx.paged_workspace(1, 1, 6, 2, 64)
+    good = ctx.paged_workspace(1, 2)
     go(good)
     ctx.finish()
     raw = abi.RlBuffer(good.raw.data, good.raw.len, good.raw.byte_len)
@@ -559,7 +589,7 @@ def test_the_workspace_is_this_contexts_and_large_enough(ctx):
     ctx.capture_begin()
     try:
         with pytest.raises(abi.RustLLMError, match="while recording"):
-            ctx.paged_workspace(1, 1, 6, 2, 64)
+            ctx.paged_workspace(1, 2)
     finally:
         ctx.graph_destroy(ctx.capture_end())
 
