@@ -685,7 +685,8 @@ class Context:
         """Attention of each request's rows of q [tokens, QH, D] over its pages
         of the [pages, KVH, page_size, D] pools.  Without a `workspace` the
         context makes and keeps its own, one for each power of two of requests
-        and KV heads (so a step to be recorded runs once before)."""
+        and KV heads (so a step to be recorded runs once before); a graph that is
+        replayed on another context needs one of its own."""
         tokens, qh, hd = q.shape
         pages, kvh, page_size, _ = k_pages.shape
         requests, blocks = table.shape

@@ -285,11 +285,14 @@ rl_status check_token_view(const char* what, const rl_buffer* b, const uint64_t*
     if (strides[2] != 1)
         return fail(RL_ERR_NON_CONTIGUOUS, "%s rows need a unit innermost stride, got %llu", what,
                     (unsigned long long)strides[2]);
-    unsigned __int128 last = 0;
-    for (int d = 0; d < 3; ++d) last += (unsigned __int128)(dims[d] - 1) * strides[d];
-    if (last >= b->len)
-        return fail(RL_ERR_INVALID_SHAPE, "%s view reaches past the end of its %llu-element buffer",
-                    what, (unsigned long long)b->len);
+    unsigned __int128 last = 0;  // below 2^64 before each sum, so none wraps
+    for (int d = 0; d < 3; ++d) {
+        last += (unsigned __int128)(dims[d] - 1) * strides[d];
+        if (last >= b->len)
+            return fail(RL_ERR_INVALID_SHAPE,
+                        "%s view reaches past the end of its %llu-element buffer", what,
+                        (unsigned long long)b->len);
+    }
     return RL_OK;
 }
 

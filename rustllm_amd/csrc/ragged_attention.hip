@@ -1633,14 +1633,17 @@ rl_status check_batch(uint64_t sequences, uint64_t tokens, uint64_t q_heads, uin
     if (kv_heads == 0 || q_heads % kv_heads != 0)
         return fail(RL_ERR_MODEL_FORMAT, "Q heads %llu must be divisible by non-zero KV heads %llu",
                     (unsigned long long)q_heads, (unsigned long long)kv_heads);
-    // a launch has fewer than 2^32 threads, at most 256 for 64 rows of all heads
+    // a launch has fewer than 2^32 threads: of the tile kernels at most 8 a row and
+    // 512 for each KV head of a request, beside 2^17 for the requests of few rows
     if (sequences > INT32_MAX || max_queries > UINT32_MAX || q_heads > kMostRows ||
         tokens > kMostRows / q_heads)
         return fail(RL_ERR_INVALID_SHAPE, "%llu rows of %llu heads exceed one launch",
                     (unsigned long long)tokens, (unsigned long long)q_heads);
-    if (sequences * kv_heads >= (uint64_t(1) << 23))
-        return fail(RL_ERR_INVALID_SHAPE, "%llu requests of %llu KV heads exceed one launch",
-                    (unsigned long long)sequences, (unsigned long long)kv_heads);
+    if (sequences * kv_heads >= (uint64_t(1) << 23) ||
+        8 * tokens * q_heads + 512 * sequences * kv_heads + (1u << 17) > UINT32_MAX)
+        return fail(RL_ERR_INVALID_SHAPE, "%llu requests of %llu KV heads exceed one launch beside %llu rows",
+                    (unsigned long long)sequences, (unsigned long long)kv_heads,
+                    (unsigned long long)(tokens * q_heads));
     if (head_dim > 512)
         return fail(RL_ERR_INVALID_SHAPE, "attention head size %llu exceeds 512",
                     (unsigned long long)head_dim);
@@ -1924,7 +1927,12 @@ rl_status workspace_entry(rl_context* ctx, uint64_t sequences, uint64_t kv_heads
     *out = rl_buffer{nullptr, 0, 0};
     if (rl_status st = check_batch(sequences, 1, kv_heads, kv_heads, 1, 1, 1.0f)) return st;
     if (rl_status st = require_context(ctx)) return st;
-    if (ctx->capturing)
+    // this context's recording, or another's that reached its stream by an event
+    hipStreamCaptureStatus recording = hipStreamCaptureStatusNone;
+    const hipError_t known = hipStreamIsCapturing(ctx->stream, &recording);
+    if (known != hipSuccess)
+        return fail(RL_ERR_DEVICE, "workspace: %s", hipGetErrorString(known));
+    if (ctx->capturing || recording != hipStreamCaptureStatusNone)
         return fail(RL_ERR_DEVICE, "a workspace cannot be made while recording a graph");
     const rl_context::Workspace size = workspace_for(ctx, sequences, kv_heads);
     const uint64_t bytes = size.ticket_bytes + size.partial_bytes;

@@ -520,8 +520,8 @@ def test_recorded_attention_follows_its_lengths(ctx, dtype, spans):
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("n", [1, 40])
 def test_pools_past_4_gib(ctx, dtype, n):
-    """Pages whose bytes and elements lie past 2^32 (32 GiB of pool in all, of which a few
-    pages are written and read)."""
+    """Pages whose bytes and elements lie past 2^32 (two pools of 18 GiB, 36 in f32, of which a
+    few pages are written and read)."""
     qh, kvh, d, page = 4, 2, 128, 64
     pages = 9 * (1 << 30) // (kvh * page * d)  # 9 Gi elements a pool
     spans = [(150, n), (70, n)]
@@ -592,6 +592,28 @@ def test_the_workspace_is_this_contexts_and_large_enough(ctx):
             ctx.paged_workspace(1, 2)
     finally:
         ctx.graph_destroy(ctx.capture_end())
+
+
+def test_no_workspace_on_a_branch_of_a_recording(ctx):
+    """A recording that another context joined by an event."""
+    fork, join = ctx.event(), ctx.event()
+    other = abi.Context(0)
+    try:
+        ctx.capture_begin()
+        try:
+            ctx.record(fork)
+            other.wait(fork)
+            with pytest.raises(abi.RustLLMError, match="while recording"):
+                other.paged_workspace(1, 2)
+            other.record(join)
+            ctx.wait(join)
+        finally:
+            ctx.graph_destroy(ctx.capture_end())
+        other.paged_workspace(1, 2).release()
+    finally:
+        other.close()
+        ctx.destroy_event(fork)
+        ctx.destroy_event(join)
 
 
 # ------------------------------------------------------------------ packed

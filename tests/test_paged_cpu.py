@@ -131,6 +131,10 @@ def test_paged_attention_validation(dt, es):
     assert st == SHAPE and "u32 slots" in msg
     st, msg = go(s=1 << 22, kvh=2)
     assert st == SHAPE and "exceed one launch" in msg
+    st, msg = go(s=1, t=127, qh=1 << 22, kvh=1 << 22, d=1)  # rows alone and heads alone would fit
+    assert st == SHAPE and "exceed one launch" in msg
+    st, msg = go(s=1 << 31, qh=1 << 29, kvh=1 << 29, t=1, d=1)
+    assert st == SHAPE and "exceed one launch" in msg
     st, msg = go(mc=1 << 31, blocks=1 << 28)
     assert st == SHAPE and "key range exceeds" in msg
     assert go(page=20)[0] == SHAPE
@@ -170,6 +174,9 @@ def test_packed_attention_validation(dt, es):
     assert go(scale=0.0)[0] == SHAPE
     assert go(offsets=buf(3, 4))[0] == SHAPE and go(offsets=buf(4, 2))[0] == DTYPE
     assert go(out=buf(3, es))[0] == SHAPE
+    most = (1 << 64) - 1  # extents whose sum passes 2^128 by six
+    st, msg = go(q=((most, 4, 8), (most, most, 1)), lens=(4096, None, None))
+    assert st == SHAPE and "reaches past the end" in msg
     st, msg = call(f"rl_packed_attention_{dt}", buf(8, es), None, None, buf(8, es), None, None,
                    buf(8, es), None, None, buf(4, 4), 3, 5, ctypes.c_float(1.0), buf(8, es))
     assert st == ARGUMENT and "null" in msg
