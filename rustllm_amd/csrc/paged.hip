@@ -32,7 +32,9 @@ namespace {
 // position of a new page is always a new token's: that token writes the
 // table entry.  Every other read of the table is of an entry that the plan
 // does not write.  Bound by latency: two dependent reads (lengths, then
-// table or free list) and the scan's two barriers.
+// table or free list) and the scan's two barriers: 3.3 us for 48 requests of one
+// token, 4.2 for 480 with 49 thousand tokens, whose call (4.7 us) takes 8.5 with a
+// workgroup for 8192 tokens instead of 1024.
 constexpr int kPlanThreads = 1024;
 constexpr int kPlanWaves = kPlanThreads / 64;
 
@@ -393,11 +395,12 @@ void launch_append(rl_context* ctx, uint64_t tokens, uint64_t heads, AppendParam
     p.packs = FastDiv(uint32_t(packs));
     // Few items: a thread a head, so that there are enough of them.  Many: four
     // heads a thread and streamed stores; from kStreamRows of rows on, more than the
-    // MALL keeps beside what is written, streamed loads too, with two heads a thread
-    // (one MI355X, 32/8 heads of 128 in f16: 2079 tokens, 26 MB of rows, 9.6 us with
-    // plain loads, 10.7 streamed, 10.3 with plain stores as well; 5663, 70 MB, 21.9 /
-    // 25.2; 8223, 101 MB, 37.2 / 35.2, 44.3).
-    const bool many = tokens * heads * packs >= uint64_t(ctx->num_cus) * 2048;
+    // MALL keeps beside what is written, streamed loads too, with two heads a thread.
+    // One MI355X, 32/8 heads of 128 in f16, a thread a head / four / two and streamed
+    // loads: 543 tokens 5.8 / 5.9 us; 1055, 6.9 / 5.9; 2079 (26 MB of rows) 10.7 / 9.6
+    // / 10.7, 10.3 with four and plain stores; 5663 (70 MB) - / 21.9 / 25.2; 8223 (101
+    // MB) - / 37.2 / 35.2, 44.3 with four and plain stores.
+    const bool many = tokens * heads * packs >= uint64_t(ctx->num_cus) * 1024;
     const bool stream = many && tokens * heads * 2 * p.half_dim * sizeof(T) >= kStreamRows;
     const uint64_t steps = ceil_div(heads, stream ? 2 : many ? 4 : 1);
     p.head_steps = FastDiv(uint32_t(steps));

@@ -186,7 +186,7 @@ __device__ inline void row_by_wave(const T* __restrict__ q, const T* __restrict_
 // Any head size up to 512, any strides and alignment: keys 256 at a time, a
 // lane's four dot products in order, the probabilities through LDS, lanes =
 // output elements for the values.  Bound by the vector ALUs and by key rows
-// read lane by lane.
+// read lane by lane: 47.7 ms for the 8 prompts that the tiles below take 0.35 ms for.
 template <typename T, int DT, bool PAGED>
 __global__ __launch_bounds__(64) void k_ragged_rows(const T* __restrict__ q,
                                                     const T* __restrict__ k,
@@ -292,7 +292,13 @@ __global__ __launch_bounds__(64) void k_ragged_rows(const T* __restrict__ q,
 // tiles are keys in the order that leaves a lane the probabilities of exactly
 // those eight rows.  A block's registers are refilled as soon as its scores (K)
 // and products (V) are through, so the next block's rows are in flight under
-// the rest of the work; its page entries are read a block ahead.  Bound by HBM.
+// the rest of the work; its page entries are read a block ahead.  Bound by HBM:
+// 155 us for 934 MB (60 requests of up to 8000 keys, 32/8 heads of 128 in f16; 6.0
+// TB/s, where a plain read runs at 6.2 to 6.4), 74.6 us for one request of 100,003
+// keys (5.5 TB/s); one request of 1536 keys takes 7.2 us, most of it the launch, three
+// dependent reads and the hand-over.  Equal shares against each request cut by
+// itself: 48.6 -> 38.7 us for 64 requests of up to 4000 keys (15/5 heads of 64).
+// Registers refilled in place leave two waves a SIMD; three spill (174 -> 243 us).
 template <typename T, int DP>
 struct SplitShape {
     static constexpr bool kHalf = std::is_same<T, half_t>::value;
@@ -665,7 +671,8 @@ __device__ inline void split_rows(const T* __restrict__ q, const T* __restrict__
         x.y *= inv;
         if (r.bad) x = make_float2(NAN, NAN);
         else if (!(fabsf(x.x) < INFINITY && fabsf(x.y) < INFINITY)) atomicOr(&odd_rows, 1u << row);
-        T* dst = out + (uint64_t(r.begin + tok) * p.q_heads + kvh * p.group + row % p.group) * hd + d;
+        T* dst = out + d +
+                 (uint64_t(r.begin + tok) * p.q_heads + kvh * p.group + row % p.group) * hd;
         dst[0] = from_float<T>(x.x);
         dst[1] = from_float<T>(x.y);
     };
@@ -763,10 +770,10 @@ __device__ inline void split_rows(const T* __restrict__ q, const T* __restrict__
 //
 // A tile is 32 QW of the rows that share a KV head (row r = token r / group,
 // head r % group of the KV head's): every K and V block serves all heads of the
-// group, and a causal tile is no longer than its 32 QW / group tokens.  Four
-// waves: QW of 32 rows times KS shares of the key blocks, merged through LDS at
-// the end.  S^T = K Q^T leaves each lane one row's scores (32 x 32 tiles), so
-// the running max and sum need one exchange between lane halves, and the
+// group, and a causal tile is no longer than its 32 QW / group tokens.  QW waves
+// of 32 rows times KS shares of the key blocks, merged through LDS at the end.
+// S^T = K Q^T leaves each lane one row's scores (32 x 32 tiles), so the running
+// max and sum need one exchange between lane halves, and the
 // probabilities come out in the operand layout of O^T += V^T P^T, the keys taken
 // in perm32 order; V's operand comes by transpose reads out of LDS.
 // K and V go from memory straight to LDS (two stages), each lane fetching 16
@@ -780,6 +787,14 @@ __device__ inline void split_rows(const T* __restrict__ q, const T* __restrict__
 // tiles, the longer ones, start first; neighbouring workgroups take
 // different KV heads, so that one XCD's workgroups (every eighth) share rows of
 // K and V in its L2.
+//
+// Bound by vector work (the softmax) beside the products, with two waves a SIMD:
+// 350 us for 8 prompts of up to 4096 tokens (32/8 heads of 128, 302 GFLOP: 860
+// TFLOP/s, where a large f16 matrix product runs at 1196), the matrix cores busy 41 %
+// of the cycles, the vector ALUs 47 %, LDS 21 % without bank conflicts.  Slower:
+// the next block's scores beside this one's softmax (356 -> 372 to 391 us), wave
+// priorities around the products (no change), 128-key blocks for head size 64 (564 -> 621 us
+// for 60 prompts).
 template <int QW>
 constexpr uint32_t kTileRows = 32 * QW;
 
@@ -841,17 +856,19 @@ __device__ inline uint32_t find_tile_request(const RaggedParams& p, uint32_t u, 
     return __builtin_amdgcn_readfirstlane(lo);
 }
 
-// Waves a SIMD that the registers leave room for: two where two workgroups of
-// four waves fit a CU's LDS.
+// Waves a SIMD that the registers have to leave room for: three for head size 128 with
+// blocks of 32 keys, else two where two workgroups of four waves fit a CU's LDS.
 template <int NT, int QW, int KS, int BN>
 constexpr int kTileWaves =
-    QW == 4 && KS == 1 && BN == 32 && NT == 4 ? 3 : QW * KS == 4 && 2 * KS * 2 * BN * (NT == 3 ? 128 : 32 * NT) * 2 <= 72 * 1024 ? 2 : 1;
+    NT == 4 && QW == 4 && BN == 32 ? 3
+    : QW * KS == 4 && 2 * KS * 2 * BN * (NT == 3 ? 128 : 32 * NT) * 2 <= 72 * 1024 ? 2
+                                                                                    : 1;
 
 // Up to 64 requests: tile u in the order of the keys that tiles see, most
 // first (in steps of a tile's tokens), so that the long ones do not start last.
-// Lane i, with request i in `r`, counts its tiles at or past a level; the tile's level is the
-// largest that u + 1 tiles reach.  Returns the request, its tile in `tile`;
-// `sequences` if there are not that many tiles.
+// Lane i, with request i in `r`, counts its tiles at or past a level; the tile's
+// level is the largest that u + 1 tiles reach.  Returns the request, its tile in
+// `tile`; `sequences` if there are not that many tiles.
 __device__ inline uint32_t find_longest_tile(const RaggedParams& p, const Request& r, uint32_t u,
                                              uint32_t rows, uint32_t& tile) {
     const uint32_t lane = threadIdx.x % 64;
@@ -1239,10 +1256,13 @@ __device__ inline void tile_rows(const half_t* __restrict__ q, const half_t* __r
 // ------------------------------------- many rows per KV head, f32 products
 //
 // The same tiles with every f32 operand as three bf16 parts (Bf16x3: six of the
-// nine products, the rest below 2^-26 of the whole), at 6/16 of the f16 rate
-// against 1/16 for f32 products of the matrix cores.  A block is 32 keys of one
-// wave, and nothing passes through LDS: K's operand is 32 bytes of a key's row
-// a lane; V's comes by columns, so a lane loads its NT elements of eight
+// nine products, the rest below 2^-26 of the whole), at a sixth of the bf16 rate
+// against a sixteenth for f32 products of the matrix cores (40.8 -> 27.5 us for 5
+// prompts of up to 1021 tokens, 9/3 heads of 64; 168 -> 84 for 6 of up to 2000 and
+// 90 -> 46 for 7 of up to 1000, 15/5 heads of 64).  Bound by the vector work
+// of the splits (51 % of the cycles; matrix cores 24 %) and few waves.  A block is
+// 32 keys of one wave, and nothing passes through LDS: K's operand is 32 bytes of a
+// key's row a lane; V's comes by columns, so a lane loads its NT elements of eight
 // neighbouring rows and splits each column across them.  K's registers are
 // refilled once the scores are through, V's after the products.
 //
@@ -1586,7 +1606,8 @@ __global__ __launch_bounds__(64 * QW * KS, (Tile<T, NT, QW, KS, BN>::kWaves)) vo
 // A paged batch of chunks and single tokens in one launch: the first
 // split_blocks workgroups stream the keys of the requests of few rows, the
 // others take tiles, so that the one's wait for memory runs beside the other's
-// products.
+// products (one MI355X: 65.5 us as two launches, 57 as one, 45.5 with the longest tiles
+// first, for 4 chunks of 509 tokens and 20 single tokens over up to 4000 keys).
 template <typename T, int NT, int QW, int KS, int BN, bool FULL>
 __global__ __launch_bounds__(64 * QW * KS, (Tile<T, NT, QW, KS, BN>::kWaves)) void k_paged_mixed(
     const T* __restrict__ q, const T* __restrict__ k, const T* __restrict__ v,
@@ -1608,8 +1629,9 @@ __global__ __launch_bounds__(64 * QW * KS, (Tile<T, NT, QW, KS, BN>::kWaves)) vo
 
 // -------------------------------------------------------------- workspace
 //
-// The split kernel's workgroups (two fit a CU: registers), their partials and
-// tickets.
+// The split kernel's workgroups (two fit a CU: registers; three or four for the
+// smaller ones of head size 64 gained nothing, 36.9 -> 38.1 / 38.9 us), their
+// partials and tickets.
 uint64_t split_slots(const rl_context* ctx, uint64_t kv_heads) {  // a KV head's
     return std::max<uint64_t>(2 * uint64_t(ctx->num_cus) / kv_heads, 1);
 }
@@ -1641,7 +1663,8 @@ rl_status check_batch(uint64_t sequences, uint64_t tokens, uint64_t q_heads, uin
                     (unsigned long long)tokens, (unsigned long long)q_heads);
     if (sequences * kv_heads >= (uint64_t(1) << 23) ||
         8 * tokens * q_heads + 512 * sequences * kv_heads + (1u << 17) > UINT32_MAX)
-        return fail(RL_ERR_INVALID_SHAPE, "%llu requests of %llu KV heads exceed one launch beside %llu rows",
+        return fail(RL_ERR_INVALID_SHAPE,
+                    "%llu requests of %llu KV heads exceed one launch beside %llu rows",
                     (unsigned long long)sequences, (unsigned long long)kv_heads,
                     (unsigned long long)(tokens * q_heads));
     if (head_dim > 512)
@@ -1698,27 +1721,47 @@ void launch_tiles(rl_context* ctx, const T* q, const T* k, const T* v, T* out,
                       p);
     }
 }
-constexpr uint64_t kSomeTiles = 100;
+// Which tiles, from the batch's 128-row tiles (`wide`) and how many of those run
+// at once (`slots`).  Measured (one MI355X, us; 15/5 heads of 64 unless another
+// head size is named, `wide` in brackets):
+//   f16, packed: QW 8 (4 for head sizes other than 64) from `slots` on, 2 x 2 below:
+//     22.6 / 16.7 [325], 50.7 / 45.6 [965], 75.7 / 75.2 [1675]; D 96 22.2 / 18.8 [261],
+//     37.7 / 36.7 [537]; D 128 21.4 / 19.2 [352], 41.7 / 44.4 [712].  Packed, QW 8
+//     against 4 at 64: 536 / 558 for 60 prompts; D 128 with blocks of 32 keys against
+//     64 (three waves a SIMD against two): 357 / 368 for 8 prompts of up to 4096.
+//     The mixed kernel does not leave the registers for either.
+//   f16, paged, whose other part takes places too: QW 4 from half of `slots` on, 2 x 2
+//     below: 55.4 / 49.2 [350], 65.2 / 76 [700]; D 128 67.5 / 71.4 [296].  Below half
+//     a tile a CU, 1 x 4 at 64: 24.6 / 28.6 [35], 32.5 / 31.8 [80], 27.2 / 30.2
+//     [115]; 40.1 / 32.6 [175].
+//   f32: 1 x 4 below a tile a CU, 2 x 2 from there on (4 x 1 for more than 64 elements):
+//     24.5 / 30.7 [155], 61.7 / 49.7 [445]; D 128 50.7 / 53.9 [144], 116 / 76.4 [352].
+// Longest tiles first (a search over the lengths in every workgroup, about 0.7 us)
+// pays where the last tiles would decide:
+//   f16, packed, `slots` to 8 `slots`: 11.1 without / 11.6 with [155], 92 / 75.8 [1675], 380 / 356
+//     [6810]; D 96 135 / 119 [1611]; D 128 41.1 / 41.7 [712], 1326 / 1402 [11 thousand]
+//   f16, paged, from 3/8 tile a CU on: 32.5 / 33.8 [80], 31.8 / 27.2 [115], 39.4 / 32.6
+//     [175]; D 128 116 / 101 [600]
+//   f32 below 4 tiles a CU: 28.9 / 27.5 [254], 50.6 / 40.9 [325], 61.4 / 62.6 [410],
+//     though 23.6 / 24.5 at [155]; more than 64 elements from a tile a CU on:
+//     48.2 / 50.7 [144], 135 / 126 [536]
 template <typename T, bool PAGED>
 void launch_tiles(rl_context* ctx, const T* q, const T* k, const T* v, T* out, RaggedParams p,
                   uint32_t sb) {
-    constexpr bool kHalf = std::is_same<T, half_t>::value;
     const uint64_t cus = uint64_t(ctx->num_cus);
     const uint64_t wide = (uint64_t(p.tokens) * p.group / kTileRows<4>) * p.kv_heads;
     const uint32_t nt = (p.head_dim + 31) / 32;
-    const uint64_t slots = (nt <= 2 ? 4 : 2) * cus;  // wide tiles at once
-    if constexpr (kHalf) {
-        p.longest_first =
-            p.sequences <= 64 && wide >= (PAGED ? kSomeTiles : slots) && wide <= 3 * slots;
-        // Packed: eight waves of 32 rows for head size 64, 32-key blocks for 128, whose
-        // registers the mixed kernel does not leave.
-        constexpr int Q64 = PAGED ? 4 : 8;
-        if (wide >= cus) {
+    if constexpr (std::is_same<T, half_t>::value) {
+        const uint64_t slots = (nt <= 2 ? 4 : 2) * cus;
+        p.longest_first = p.sequences <= 64 && wide >= (PAGED ? 3 * cus / 8 : slots) &&
+                          wide <= 8 * slots;
+        if (wide >= (PAGED ? slots / 2 : slots)) {
             if (nt == 1) launch_tiles<T, 1, 4, 1, 64, PAGED>(ctx, q, k, v, out, p, sb);
-            else if (nt == 2) launch_tiles<T, 2, Q64, 1, 64, PAGED>(ctx, q, k, v, out, p, sb);
+            else if (nt == 2)
+                launch_tiles<T, 2, PAGED ? 4 : 8, 1, 64, PAGED>(ctx, q, k, v, out, p, sb);
             else if (nt == 3) launch_tiles<T, 3, 4, 1, 64, PAGED>(ctx, q, k, v, out, p, sb);
             else launch_tiles<T, 4, 4, 1, PAGED ? 64 : 32, PAGED>(ctx, q, k, v, out, p, sb);
-        } else if (PAGED && nt == 2 && wide < kSomeTiles) {
+        } else if (PAGED && nt == 2 && wide < cus / 2) {
             launch_tiles<T, 2, 1, 4, 32, PAGED>(ctx, q, k, v, out, p, sb);
         } else {
             if (nt == 1) launch_tiles<T, 1, 2, 2, 64, PAGED>(ctx, q, k, v, out, p, sb);
@@ -1727,13 +1770,13 @@ void launch_tiles(rl_context* ctx, const T* q, const T* k, const T* v, T* out, R
             else launch_tiles<T, 4, 2, 2, 32, PAGED>(ctx, q, k, v, out, p, sb);
         }
     } else {
-        p.longest_first = p.sequences <= 64 && wide < 4 * cus;
-        if (nt >= 3 && wide >= cus) {
-            if (nt == 3) launch_tiles<T, 3, 4, 1, 32, PAGED>(ctx, q, k, v, out, p, sb);
-            else launch_tiles<T, 4, 4, 1, 32, PAGED>(ctx, q, k, v, out, p, sb);
-        } else if (wide >= cus) {
+        p.longest_first =
+            p.sequences <= 64 && wide >= (nt >= 3 ? cus : 0) && wide < 4 * cus;
+        if (wide >= cus) {
             if (nt == 1) launch_tiles<T, 1, 2, 2, 32, PAGED>(ctx, q, k, v, out, p, sb);
-            else launch_tiles<T, 2, 2, 2, 32, PAGED>(ctx, q, k, v, out, p, sb);
+            else if (nt == 2) launch_tiles<T, 2, 2, 2, 32, PAGED>(ctx, q, k, v, out, p, sb);
+            else if (nt == 3) launch_tiles<T, 3, 4, 1, 32, PAGED>(ctx, q, k, v, out, p, sb);
+            else launch_tiles<T, 4, 4, 1, 32, PAGED>(ctx, q, k, v, out, p, sb);
         } else {
             if (nt == 1) launch_tiles<T, 1, 1, 4, 32, PAGED>(ctx, q, k, v, out, p, sb);
             else if (nt == 2) launch_tiles<T, 2, 1, 4, 32, PAGED>(ctx, q, k, v, out, p, sb);
@@ -1912,7 +1955,9 @@ rl_status paged_entry(rl_context* ctx, const char* name, const rl_buffer* q,
             launch_split<T>(ctx, qd, kd, vd, od, p);
             return after_launch(ctx, name);
         }
-        // beside tiles: half of the workgroups that would fill the CUs
+        // beside tiles: half of the workgroups that would fill the CUs (60 single tokens of
+        // up to 8000 keys and a chunk of 30 tokens: 183 us, a quarter 295; 4 chunks and
+        // 20 single tokens of up to 4000 keys: 57 / 56)
         p.slots = uint32_t(std::max<uint64_t>(slots / 2, 1));
         split_blocks = p.slots * p.kv_heads;
     }

@@ -315,6 +315,10 @@ PAGED = [
     ([(70, 500), (0, 310), (5, 1), (300, 300)], 32, 8, 96, 16),
     ([(70, 500), (0, 310), (5, 3), (300, 300)], 32, 8, 32, 64),
     ([(40, 200), (0, 310), (5, 1), (1300, 290)], 15, 5, 64, 16),
+    ([(40, 300), (0, 310), (5, 1), (1300, 290)], 15, 5, 64, 16),
+    *[([(100, 300), (0, 310), (700, 290), (5, 1), (33, 300)], 64, 16, d, 16)
+      for d in (64, 56, 32, 24)],
+    *[([(100, 300), (0, 310), (5, 2), (300, 450)], 32, 8, d, 32) for d in (112, 80)],
 ]
 
 
@@ -688,6 +692,8 @@ PACKED = [
     ([700, 500, 33, 64], 32, 8, 64), ([600, 511, 1], 32, 8, 128), ([400, 700], 32, 8, 96),
     ([900, 300], 32, 8, 32), ([260, 30, 511] * 6, 32, 8, 64), ([130, 300] * 10, 32, 8, 128),
     ([40] * 80 + [900], 32, 8, 64),
+    *[([700, 500, 33, 64, 300, 500], 64, 16, d) for d in (64, 56, 32, 24)],
+    *[([600, 511, 1], 64, 16, d) for d in (128, 112, 96, 80)],
 ]
 
 
