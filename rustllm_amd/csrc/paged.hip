@@ -33,8 +33,8 @@ namespace {
 // table entry.  Every other read of the table is of an entry that the plan
 // does not write.  Bound by latency: two dependent reads (lengths, then
 // table or free list) and the scan's two barriers: 3.3 us for 48 requests of one
-// token, 4.2 for 480 with 49 thousand tokens, whose call (4.7 us) takes 8.5 with a
-// workgroup for 8192 tokens instead of 1024.
+// token, 4.4 for 480 with 49 thousand tokens (a call 4.7; 8.5 with a workgroup for
+// 8192 tokens instead of 1024).
 constexpr int kPlanThreads = 1024;
 constexpr int kPlanWaves = kPlanThreads / 64;
 

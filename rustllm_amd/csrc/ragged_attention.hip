@@ -297,7 +297,7 @@ __global__ __launch_bounds__(64) void k_ragged_rows(const T* __restrict__ q,
 // TB/s, where a plain read runs at 6.2 to 6.4), 74.6 us for one request of 100,003
 // keys (5.5 TB/s); one request of 1536 keys takes 7.2 us, most of it the launch, three
 // dependent reads and the hand-over.  Equal shares against each request cut by
-// itself: 48.6 -> 38.7 us for 64 requests of up to 4000 keys (15/5 heads of 64).
+// itself: 44 -> 40 us for 64 requests of up to 4000 keys (15/5 heads of 64).
 // Registers refilled in place leave two waves a SIMD; three spill (174 -> 243 us).
 template <typename T, int DP>
 struct SplitShape {
