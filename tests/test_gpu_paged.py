@@ -522,6 +522,103 @@ def test_recorded_attention_follows_its_lengths(ctx, dtype, spans):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
+def test_recorded_steps_share_tables_pages_and_a_workspace(ctx, dtype):
+    """Whole steps (plan, append, attention) as two graphs, one of single tokens
+    and one of chunks, over the same requests: replayed in turn with the lengths
+    and free pages of each step, against the same calls run eagerly on a copy of
+    the tables and pools, bit for bit."""
+    qh, kvh, d, page, blocks, pages, requests = 6, 2, 64, 16, 24, 60, 3
+    heads = qh + 2 * kvh
+    angle = np.arange(400)[:, None] * 100.0 ** (-np.arange(0, d, 2) / d)[None]
+    cos, sin = (ctx.upload(f(angle).astype(np.float32)) for f in (np.cos, np.sin))
+    state = [ctx.upload(np.full((requests, blocks), NONE, np.uint32)),
+             *(ctx.upload(np.full((pages, kvh, page, d), np.nan, dtype)) for _ in range(2))]
+    mirror = [ctx.clone(b) for b in state]
+    u32 = lambda v: ctx.upload(np.array(v, np.uint32))
+
+    class Step:
+        def __init__(self, rows, chunk):
+            self.rows, self.chunk = rows, chunk
+            self.cached, self.fresh, self.free = u32([0] * 3), u32([0] * 3), u32([NONE] * pages)
+            self.x = ctx.empty((rows, heads, d), dtype)
+            self.planned = [ctx.empty((n,), np.uint32) for n in (requests + 1, requests, rows,
+                                                                 rows, 1)]
+            self.q, self.out = (ctx.empty((rows, qh, d), dtype) for _ in range(2))
+
+        def run(self, state):
+            table, dk, dv = state
+            offsets, context, slots, positions, taken = self.planned
+            ctx.paged_plan(self.cached, self.fresh, self.free, table, page, pages, offsets,
+                           context, slots, positions, taken)
+            views = [(View(ctx, abi.RlBuffer(self.x.raw.data + first * d * self.x.dtype.itemsize,
+                                             self.x.len - first * d,
+                                             self.x.byte_len - first * d * self.x.dtype.itemsize),
+                           dtype, (self.x.len - first * d,)),
+                      (self.rows, n, d), (heads * d, d, 1))
+                     for first, n in ((0, qh), (qh, kvh), (qh + kvh, kvh))]
+            ctx.qkv_rope_paged_append(*views, cos, sin, positions, slots, dk, dv, self.q)
+            ctx.paged_attention(self.q, dk, dv, table, offsets, context, 0.125, self.chunk,
+                                blocks * page, self.out)
+
+        def results(self):
+            return [b.numpy() for b in (*self.planned, self.out)]
+
+    steps = {"one": Step(4, 2), "chunk": Step(90, 70)}
+    graphs = {}
+    for name, step in steps.items():
+        step.run(state)  # three idle requests: makes the workspace, writes no page
+        ctx.finish()
+        ctx.capture_begin()
+        step.run(state)
+        graphs[name] = ctx.capture_end()
+    cached, free = [0] * requests, list(np.random.default_rng(3).permutation(pages))
+    try:
+        for turn, (name, fresh) in enumerate([
+                ("chunk", [60, 0, 7]), ("one", [1, 1, 1]), ("one", [1, 1, 2]),
+                ("chunk", [1, 66, 1]), ("one", [0, 1, 1]), ("chunk", [70, 3, 17]),
+                ("one", [1, 1, 1]), ("chunk", [0, 0, 0]), ("one", [2, 0, 1])]):
+            step = steps[name]
+            for buffer, value in ((step.cached, cached), (step.fresh, fresh),
+                                  (step.free, free + [NONE] * (pages - len(free)))):
+                ctx.copy(u32(value), buffer)
+            ctx.copy(ctx.upload(normal((step.rows, heads, d), dtype, "step", turn)), step.x)
+            ctx.copy(ctx.upload(np.full((step.rows, qh, d), 7.0, dtype)), step.out)
+            ctx.graph_launch(graphs[name])
+            ctx.finish()
+            replayed = step.results()
+            ctx.copy(ctx.upload(np.full((step.rows, qh, d), 7.0, dtype)), step.out)
+            step.run(mirror)
+            ctx.finish()
+            for i, (got, want) in enumerate(zip(replayed, step.results())):
+                assert_bitexact(got, want, f"turn {turn} output {i}")
+            for got, want in zip(state, mirror):
+                assert_bitexact(got.numpy(), want.numpy(), f"turn {turn} tables and pages")
+            total = sum(fresh)
+            assert np.isfinite(replayed[-1]).all() and np.all(replayed[-1][total:] == 7.0)
+            assert total == 0 or not np.any(np.all(replayed[-1][:total] == 7.0, axis=(1, 2)))
+            cached = [c + n for c, n in zip(cached, fresh)]
+            free = free[int(replayed[4][0]):]
+    finally:
+        for graph in graphs.values():
+            ctx.graph_destroy(graph)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("n", [1, 40])
+def test_requests_share_a_prefix_behind_rows_of_none(ctx, dtype, n):
+    """Two requests whose first pages are the same ones; the batch's first rows
+    belong to no request."""
+    b = Batch([(100, n), (130, 1), (99, n)], 6, 2, 64, 16, dtype, ("prefix", n), padding=5)
+    b.table[1, :6] = b.table[0, :6]
+    for x in (b.k, b.v):
+        x[1][:96] = x[0][:96]
+    b.offsets += 2
+    got = b.run(ctx)
+    b.check(got)
+    assert np.all(got[:2] == 7.0)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("n", [1, 40])
 def test_pools_past_4_gib(ctx, dtype, n):
     """Pages whose bytes and elements lie past 2^32 (two pools of 18 GiB, 36 in f32, of which a
