@@ -375,6 +375,10 @@ __device__ inline uint32_t wave_scan(uint32_t v) {  // inclusive sum
 __device__ inline uint32_t last_lane(uint32_t v) {
     return uint32_t(__builtin_amdgcn_readlane(int(v), 63));
 }
+__device__ inline uint64_t wide_of_lane(uint64_t v, int at) {
+    return uint64_t(uint32_t(__builtin_amdgcn_readlane(int(v >> 32), at))) << 32 |
+           uint32_t(__builtin_amdgcn_readlane(int(v), at));
+}
 
 // FULL: the head size is DP; else it is a smaller multiple of 16 bytes and the
 // operands' elements past it are zeros (K, Q) or any row's own (V, whose output
@@ -408,46 +412,78 @@ __device__ inline void split_rows(const T* __restrict__ q, const T* __restrict__
     const uint32_t kvh = block % p.kv_heads;
     const uint64_t w = block / p.kv_heads;
 
-    // Every workgroup's share of the units: `per` of them in request order.
-    Request lane0;  // of the first 64 requests
-    const uint32_t units0 = split_units(p, lane, kUnitShift, lane0);
-    const uint32_t upto0 = wave_scan(units0);
-    uint64_t total = last_lane(upto0);
-    Request other;
-    for (uint32_t base = 64; base < p.sequences; base += 64)
-        total += last_lane(wave_scan(split_units(p, base + lane, kUnitShift, other)));
+    // Every workgroup's share of the units: `per` of them in request order.  The
+    // share's requests come in windows of 64, a lane each: `base` is the window's
+    // first request, `before` the units of those before it.
+    uint32_t base = 0, units_here, upto;
+    uint64_t before = 0;
+    Request here;
+    auto load_window = [&] {
+        units_here = split_units(p, base + lane, kUnitShift, here);
+        upto = wave_scan(units_here);
+    };
+    uint64_t total, group_before = 0, group_upto = 0;
+    const uint32_t run = (p.sequences + 64 * kSplitWaves - 1) / (64 * kSplitWaves);
+    if (p.sequences <= 64) {
+        load_window();
+        total = last_lane(upto);
+    } else {
+        // more: each thread sums `run` requests, a lane then four threads' sums (256
+        // requests of up to 300 keys, 15/5 heads of 64: 20.8 us, 26.4 where every request
+        // was looked for from the first on; 4096: 226 / 1183)
+        uint64_t* sums = reinterpret_cast<uint64_t*>(&lds.o[0][0][0]);
+        uint64_t sum = 0;
+        const uint64_t from = uint64_t(threadIdx.x) * run;
+#pragma unroll 4
+        for (uint32_t i = 0; i < run; ++i)
+            sum += split_units(p, uint32_t(min(from + i, uint64_t(p.sequences))), kUnitShift, here);
+        sums[threadIdx.x] = sum;
+        __syncthreads();
+        uint64_t four = 0;
+#pragma unroll
+        for (int i = 0; i < kSplitWaves; ++i) four += sums[kSplitWaves * lane + i];
+        group_upto = four;
+#pragma unroll
+        for (int d = 1; d < 64; d *= 2) {
+            const uint64_t lower = __shfl_up(group_upto, d, 64);
+            group_upto += int(lane) >= d ? lower : 0u;
+        }
+        group_before = group_upto - four;
+        total = wide_of_lane(group_upto, 63);
+    }
     const uint64_t per = max(uint64_t(1), (total + p.slots - 1) / p.slots);
     const uint64_t end = min(total, (w + 1) * per);
     // Keys and values that the MALL does not keep between layers or steps anyway
     // are streamed past it (one MI355X: 934 MB 172 / 165 us, 410 MB 83.3 / 79.8, 164
     // MB 38.7 / 37.9; 50 MB 16.5 / 18.4).
     const bool stream = total * kUnit * p.kv_heads * 2 * (hd * sizeof(T)) >= kStreamKeyBytes;
+    if (w * per >= end) return;
+    if (p.sequences > 64) {  // the share's first window
+        const int in = __builtin_ctzll(__ballot(group_upto > w * per));
+        base = uint32_t(in) * kSplitWaves * run;
+        before = wide_of_lane(group_before, in);
+        load_window();
+    }
     for (uint64_t at = w * per; at < end;) {
     // the request of unit `at`: the first whose units end past it
-    uint32_t request = 0, units = 0;
-    uint64_t first = 0;  // its first unit
-    Request r{};
-    for (uint32_t base = 0; base < p.sequences; base += 64) {
-        other = lane0;
-        const uint32_t mine =
-            base == 0 ? units0 : split_units(p, base + lane, kUnitShift, other);
-        const uint32_t upto = base == 0 ? upto0 : wave_scan(mine);
-        const uint64_t past = __ballot(first + upto > at);
-        if (past != 0) {
-            const int in = __builtin_ctzll(past);
-            request = base + in;
-            units = uint32_t(__builtin_amdgcn_readlane(int(mine), in));
-            first += uint32_t(__builtin_amdgcn_readlane(int(upto), in)) - units;
-            r = request_of_lane(other, in);
-            break;
-        }
-        first += last_lane(upto);
+    uint64_t past = __ballot(before + upto > at);
+    while (past == 0 && base + 64 < p.sequences) {
+        before += last_lane(upto);
+        base += 64;
+        load_window();
+        past = __ballot(before + upto > at);
     }
+    const int in = past == 0 ? 0 : __builtin_ctzll(past);
+    const uint32_t request = base + in;
+    const uint32_t units = uint32_t(__builtin_amdgcn_readlane(int(units_here), in));
+    const uint64_t first =  // its first unit
+        before + uint32_t(__builtin_amdgcn_readlane(int(upto), in)) - units;
+    const Request r = request_of_lane(here, in);
     const uint64_t w0 = first / per;  // workgroups w0 .. w0 + n_splits - 1 share the request
     const uint32_t n_splits = uint32_t((first + units - 1) / per - w0) + 1;
     const uint32_t split = uint32_t(w - w0);
     const uint32_t u0 = uint32_t(at - first), u1 = uint32_t(min(uint64_t(units), end - first));
-    at = first + u1;
+    at = max(at + 1, first + u1);  // (whatever the lengths, an end)
     const uint32_t R = r.n * p.group;
     const uint32_t last = r.keys == 0 ? 0u : r.keys - 1;
     const uint32_t blocks = r.bad ? 0u : (r.keys + kKeys - 1) / kKeys;

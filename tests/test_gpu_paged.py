@@ -344,6 +344,21 @@ def test_paged_attention_of_many_requests(ctx, dtype):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("requests,chunk", [(64, 2), (65, 2), (257, 2), (257, 40), (1500, 2),
+                                            (5000, 1)])
+def test_paged_attention_finds_its_requests(ctx, dtype, requests, chunk):
+    """Many requests of a few keys, runs of idle ones and a long one among them."""
+    rng = np.random.default_rng(requests + chunk)
+    spans = [(int(c), int(n)) for c, n in zip(rng.integers(0, 40, requests),
+                                              rng.integers(0, chunk + 1, requests))]
+    idle = slice(requests // 5, requests // 5 + 100 if requests > 200 else requests // 5 + 9)
+    spans[idle] = [(c, 0) for c, _ in spans[idle]]
+    spans[requests // 2], spans[-1] = (3000, 1), (0, 1)
+    b = Batch(spans, 6, 2, 64, 16, dtype, ("requests", requests, chunk), padding=1)
+    b.check(b.run(ctx))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
 def test_paged_attention_bounds_may_be_loose(ctx, dtype):
     """max_queries, max_context and the table row far above what the batch has."""
     b = Batch([(100, 1), (7, 1), (40, 1)], 9, 3, 64, 16, dtype, ("loose",), blocks=4096)
