@@ -549,7 +549,10 @@ rl_status rl_gqa_pv_matmul_f16(rl_context* ctx, const rl_buffer* probs, const rl
  * step follows what its replay finds in them.  Row ranges, pages and slots
  * that lie outside their buffers are never followed (each entry says what
  * comes out).  The batch's tokens are rows: request i owns rows offsets[i] ..
- * offsets[i + 1] of every [tokens, heads, head_dim] tensor. */
+ * offsets[i + 1] of every [tokens, heads, head_dim] tensor.  An attention call
+ * is one launch and refused past its size: 8 tokens q_heads + 512 sequences
+ * kv_heads + 2^17 up to 2^32 - 1, and tokens q_heads below 2^26 where head size,
+ * strides, alignment or pages of fewer than 8 rows rule the matrix cores out. */
 #define RL_NO_PAGE 0xffffffffu
 #define RL_NO_SLOT 0xffffffffu
 
