@@ -81,14 +81,6 @@ __device__ inline float max_halves(float v) {
     return fmaxf(__uint_as_float(s[0]), __uint_as_float(s[1]));
 }
 
-// max(a, b, c) in one v_max3_f32.  (fmaxf on a value the compiler cannot
-// prove canonical, such as an MFMA result, costs an extra v_max_f32 x, x.)
-__device__ inline float max3(float a, float b, float c) {
-    float r;
-    asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "v"(c));
-    return r;
-}
-
 // Buffer resource (gfx9 descriptor: base, stride 0, size in bytes, 32-bit
 // data format) for raw loads from `base`: a load at or past `bytes` returns
 // zeros.

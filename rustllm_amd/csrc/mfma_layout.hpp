@@ -62,6 +62,15 @@ __device__ inline h4 lds_read_transposed(const half_t* p) {
     return __builtin_bit_cast(h4, r);
 }
 
+// max(a, b, c) in one v_max3_f32, a NaN passed over.  Of matrix-product results: the
+// number maximum needs no v_max_f32 x, x before it (fmaxf does, for a value that
+// may be a signalling NaN), and the compiler sees it, so the wait states that an
+// MFMA's result asks for before a vector read are there.  In inline assembly they
+// are not: the compiler counts them for its own instructions only.
+__device__ inline float max3(float a, float b, float c) {
+    return __builtin_elementwise_maximumnum(__builtin_elementwise_maximumnum(a, b), c);
+}
+
 // f32 products on the bf16 matrix cores (v_mfma_f32_32x32x16_bf16, 16 times
 // the rate of the f32 ones).  An f32 value is the sum of three bf16 parts, each
 // the rounding of what the parts before it leave (8 + 8 + 8 bits, and their

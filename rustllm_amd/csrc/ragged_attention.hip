@@ -857,14 +857,6 @@ __device__ inline float halves_max(float v) {
                                                     false);
     return fmaxf(__uint_as_float(s[0]), __uint_as_float(s[1]));
 }
-// max(a, b, c) as one instruction (fmaxf would first canonicalise what comes
-// out of a matrix product)
-__device__ inline float max3(float a, float b, float c) {
-    float r;
-    asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "v"(c));
-    return r;
-}
-
 // Zeros for the chunks of a padded K row.
 __device__ __align__(16) const uint32_t zero_chunk[4] = {0, 0, 0, 0};
 
