@@ -28,6 +28,14 @@ namespace {
 
 constexpr float kLog2e = 1.44269504088896340736f;
 
+// Added to the exponent of a probability that is rounded to f16, in the sum as in
+// the product, so that it cancels in their quotient: f16's normal range then reaches
+// down to 2^-26 of the row's maximum, and what is rounded away below it is at most
+// 2^-37 of that a key (2^-25 without: over 100 thousand keys of 2^-27 each beside one
+// of weight 1, 7e-4 of the whole).  The largest, kSlack past the maximum, is 2^15,
+// below f16's 65504.
+constexpr float kRaise = 12.0f;
+
 struct RaggedParams {
     const uint32_t* offsets;  // [sequences + 1]
     const uint32_t* context;  // [sequences] (paged)
@@ -605,6 +613,7 @@ __device__ inline void split_rows(const T* __restrict__ q, const T* __restrict__
         const float m_new = fmaxf(m, mx);
         const float shift = m_new == -INFINITY ? 0.0f : m_new;
         const float alpha = __builtin_amdgcn_exp2f(m - shift);
+        const float neg_m = (kHalf ? kRaise : 0.0f) - shift;
         m = m_new;
         l *= alpha;
 #pragma unroll
@@ -615,7 +624,7 @@ __device__ inline void split_rows(const T* __restrict__ q, const T* __restrict__
         for (int t = 0; t < S::kKTiles; ++t)
 #pragma unroll
             for (int e = 0; e < 4; ++e)
-                s[t][e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[t][e], p.scale_log2, -shift));
+                s[t][e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[t][e], p.scale_log2, neg_m));
     };
     auto values = [&] {
         if constexpr (kHalf) {
@@ -861,7 +870,8 @@ __device__ inline float halves_max(float v) {
 __device__ __align__(16) const uint32_t zero_chunk[4] = {0, 0, 0, 0};
 
 // A row's running max (log2 units) moves only when a block passes it by more
-// than this: probabilities stay below 2^3, and most blocks skip the rescaling.
+// than this: probabilities stay below 2^3 (f16: times 2^kRaise), and most blocks skip
+// the rescaling.
 constexpr float kSlack = 3.0f;
 
 // Tile u's request: the last one whose first tile is not past u (64 candidates
@@ -1186,7 +1196,7 @@ __device__ inline void tile_rows(const half_t* __restrict__ q, const half_t* __r
 #pragma unroll
                     for (int e = 0; e < 16; ++e) o[t][e] *= alpha;
             }
-            const float neg_m = m == -INFINITY ? 0.0f : -m;
+            const float neg_m = (m == -INFINITY ? 0.0f : -m) + kRaise;
             // the sum adds the same rounded probabilities that the product takes
             const h2 ones = {half_t(1.0f), half_t(1.0f)};
             h8 pb[BN / 16];

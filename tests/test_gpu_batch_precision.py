@@ -56,3 +56,89 @@ def test_attention_of_very_wide_scores(ctx, dtype, sigma, qh, kvh, q_len, kv_len
     err = np.abs(got - exact)
     worst = np.unravel_index(np.argmax(err / bound), err.shape)
     assert np.all(err <= bound), f"error {err[worst]:.3g} > {bound[worst]:.3g} at {worst}"
+
+
+def heavy_and_light(spans, qh, kvh, d, dtype, light, key):
+    """A batch whose every row sees one key of weight 1, whose values are zeros, and, of each
+    other key, 2^light of that weight (to f16's steps of the scores), values of about 1."""
+    b = Batch(spans, qh, kvh, d, 64, dtype, key)
+    b.q[:] = 0.0
+    b.q[:, :, 0] = np.sqrt(d)  # the score is the key's first element
+    for i, keys in enumerate(b.context):
+        k, v = b.k[i], b.v[i]
+        k[:, :, 0] = 8.0 + light * np.log(2.0)
+        v[:] = (1.0 + 0.125 * v.astype(np.float32)).astype(dtype)
+        k[spans[i][0] // 3, :, 0], v[spans[i][0] // 3] = 8.0, 0.0
+        pos = np.arange(keys)
+        b.kp[b.table[i, pos // 64], :, pos % 64] = k
+        b.vp[b.table[i, pos // 64], :, pos % 64] = v
+    b.scale = 1.0 / np.sqrt(d)
+    return b
+
+
+def check_light_weights(b, got):
+    """As attention_bound, but for its kv_len 2^-25 max|v| of f16 probabilities below the
+    normal range: each is raised by 2^12 over the row's maximum, which leaves
+    kv_len 2^-37 max|v|."""
+    for i in range(len(b.spans)):
+        rows, exact, bound = b.expect(i)
+        if b.q.dtype == np.float16:
+            vmax = np.max(np.abs(b.v[i].astype(np.float64)))
+            bound = bound - int(b.context[i]) * (2.0 ** -25 - 2.0 ** -37) * vmax
+        err = np.abs(got[rows].astype(np.float64).transpose(1, 0, 2) - exact)
+        worst = np.unravel_index(np.argmax(err / bound), err.shape)
+        assert np.all(err <= bound), (f"request {i}: error {err[worst]:.3g} > {bound[worst]:.3g} "
+                                      f"of {exact[worst]:.3g} at {worst}")
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("n", [1, 20])
+@pytest.mark.parametrize("d", [64, 128, 96, 80, 32])
+@pytest.mark.parametrize("light", [-12.0, -16.5, -21.3, -27.4])
+def test_many_light_keys_keep_their_weight(ctx, dtype, light, d, n):
+    """One heavy key among a hundred thousand, and among thirty thousand, light ones."""
+    b = heavy_and_light([(100000, n), (30001, 1)], 2, 1, d, dtype, light, ("light", d, n))
+    check_light_weights(b, b.run(ctx))
+
+
+@pytest.mark.parametrize("d", [64, 128, 96, 80, 32])
+@pytest.mark.parametrize("light", [-10.0, -14.5, -16.5, -20.3])
+def test_light_keys_of_a_packed_prompt(ctx, light, d):
+    """The same within a prompt (f16): the heavy key is its first token."""
+    tokens = 3000
+    q, k, v = (np.zeros((tokens, 1, d), np.float16) for _ in range(3))
+    q[:, :, 0] = np.sqrt(d)
+    k[:, :, 0] = 8.0 + light * np.log(2.0)
+    v[:] = 1.0 + 0.125 * normal(v.shape, np.float32, "light packed", d)
+    k[0, :, 0], v[0] = 8.0, 0.0
+    scale = 1.0 / np.sqrt(d)
+    view = lambda x: (ctx.upload(x), x.shape, (d, d, 1))
+    offsets = ctx.upload(np.array([0, tokens], np.uint32))
+    got = ctx.packed_attention(view(q), view(k), view(v), offsets, scale, tokens).numpy()
+    rows = np.r_[0:3, 31:34, 1000:1003, 2990:3000]
+    for r in rows:
+        exact, bound = attention_bound(q[r][None, None], k[:r + 1].transpose(1, 0, 2)[None],
+                                       v[:r + 1].transpose(1, 0, 2)[None], scale, int(r), None,
+                                       "f16_fused")
+        vmax = np.max(np.abs(v[:r + 1].astype(np.float64)))
+        bound = bound[0, :, 0] - (r + 1) * (2.0 ** -25 - 2.0 ** -37) * vmax
+        err = np.abs(got[r].astype(np.float64) - exact[0, :, 0])
+        assert np.all(err <= bound), (int(r), float(np.max(err / bound)))
+
+
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("q_len", [1, 300])
+def test_light_keys_of_one_sequence(ctx, q_len, d):
+    """rl_attention_f16, whose probabilities stop at f16's own range: weights of 2^-16.5,
+    in which its sum and its product have to agree."""
+    keys = 30000
+    q, k, v = np.zeros((1, 2, q_len, d)), np.zeros((1, 1, keys, d)), np.ones((1, 1, keys, d))
+    q[..., 0], k[..., 0] = np.sqrt(d), 8.0 - 16.5 * np.log(2.0)
+    k[:, :, 5, 0], v[:, :, 5] = 8.0, 0.0
+    q, k, v = (x.astype(np.float16) for x in (q, k, v))
+    got = ctx.attention(ctx.upload(q), ctx.upload(k), ctx.upload(v), 1.0 / np.sqrt(d),
+                        keys - q_len).numpy().astype(np.float64)
+    exact, bound = attention_bound(q[:, :, :1], k[:, :, :keys - q_len + 1],
+                                   v[:, :, :keys - q_len + 1], 1.0 / np.sqrt(d), keys - q_len,
+                                   None, "f16_fused")
+    assert np.all(np.abs(got[:, :, :1] - exact) <= bound)
