@@ -617,8 +617,9 @@ rl_status rl_paged_attention_workspace(rl_context* ctx, uint64_t sequences, uint
  * are not written; a row that sees no key (a position below 0) is zeros; a
  * row that sees a key of a page at or past `pages`, and every row of a
  * request whose context passes max_context, is NaN.  Types, roundings and
- * head sizes as rl_attention_*.  May be recorded into a graph, the workspace
- * made before. */
+ * head sizes as rl_attention_*; the f16 probabilities of requests of up to 16
+ * rows a KV head (rows times q_heads / kv_heads) have 22 bits for every head
+ * size.  May be recorded into a graph, the workspace made before. */
 rl_status rl_paged_attention_f32(rl_context* ctx, const rl_buffer* q, const rl_buffer* k_pages,
                                  const rl_buffer* v_pages, const rl_buffer* block_table,
                                  const rl_buffer* offsets, const rl_buffer* context,

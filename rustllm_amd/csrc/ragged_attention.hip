@@ -293,6 +293,11 @@ __global__ __launch_bounds__(64) void k_ragged_rows(const T* __restrict__ q,
 // sum over the requests.  Requests that lie in several shares leave partials,
 // which meet by a ticket: the workgroup that finishes last merges them.
 //
+// The probabilities of f16 enter the second product as the sum of two f16 parts, 22
+// bits, which its matrix cores have the time for: with one part the mean error against
+// 64 bits was 2.57e-4 of the outputs' for 60 requests of up to 8000 keys, with two 1.77e-4,
+// that of the outputs' own rounding, at the same 155 us (head size 32: 39.1 -> 40.5).
+//
 // Layout: K's operand is its rows as they lie in memory (16 bytes a lane).  V's
 // has to come by columns: a lane loads its 4 or 8 columns of eight
 // neighbouring rows (f32: of four) and takes the operand of each column across
@@ -630,17 +635,20 @@ __device__ inline void split_rows(const T* __restrict__ q, const T* __restrict__
         if constexpr (kHalf) {
 #pragma unroll
             for (int t = 0; t < S::kVSteps; ++t) {
-                h8 pb;
+                h8 pb, pl;  // high and low parts: 22 bits
 #pragma unroll
                 for (int e = 0; e < 8; ++e) {
-                    pb[e] = half_t(s[2 * t + e / 4][e % 4]);
-                    l += float(pb[e]);  // the sum of the rounded ones, as the product takes them
+                    const float x = s[2 * t + e / 4][e % 4];
+                    pb[e] = half_t(x);
+                    pl[e] = half_t(x - float(pb[e]));
+                    l += x;
                 }
 #pragma unroll
                 for (int c = 0; c < S::kTiles; ++c) {
                     h8 va;
 #pragma unroll
                     for (int e = 0; e < 8; ++e) va[e] = x.v[t][e][0][c];
+                    o[c] = __builtin_amdgcn_mfma_f32_16x16x32_f16(va, pl, o[c], 0, 0, 0);
                     o[c] = __builtin_amdgcn_mfma_f32_16x16x32_f16(va, pb, o[c], 0, 0, 0);
                 }
             }
@@ -821,6 +829,9 @@ __device__ inline void split_rows(const T* __restrict__ q, const T* __restrict__
 // max and sum need one exchange between lane halves, and the
 // probabilities come out in the operand layout of O^T += V^T P^T, the keys taken
 // in perm32 order; V's operand comes by transpose reads out of LDS.
+// Head sizes off the multiples of 32 (!FULL) have probabilities of two f16 parts, as
+// rl_attention_f16's: 22 bits (one part took 39.2 us where two take 45.2, 10 prompts of up
+// to 1600, 32/8 heads of 80, and 115 where they take 149, 8 of up to 3000 with heads of 112).
 // K and V go from memory straight to LDS (two stages), each lane fetching 16
 // bytes from an address of its own -- its key's row, wherever its page is --
 // the page entries read a step ahead.  Keys past the request's last read that
@@ -1199,16 +1210,24 @@ __device__ inline void tile_rows(const half_t* __restrict__ q, const half_t* __r
             const float neg_m = (m == -INFINITY ? 0.0f : -m) + kRaise;
             // the sum adds the same rounded probabilities that the product takes
             const h2 ones = {half_t(1.0f), half_t(1.0f)};
-            h8 pb[BN / 16];
+            h8 pb[BN / 16], pl[FULL ? 1 : BN / 16];
 #pragma unroll
             for (int c = 0; c < BN / 16; ++c) {
 #pragma unroll
-                for (int e = 0; e < 8; ++e)
-                    pb[c][e] = half_t(__builtin_amdgcn_exp2f(
-                        __builtin_fmaf(s[c / 2][8 * (c % 2) + e], p.scale_log2, neg_m)));
+                for (int e = 0; e < 8; ++e) {
+                    const float x = __builtin_amdgcn_exp2f(
+                        __builtin_fmaf(s[c / 2][8 * (c % 2) + e], p.scale_log2, neg_m));
+                    pb[c][e] = half_t(x);
+                    if constexpr (!FULL) {
+                        pl[c][e] = half_t(x - float(pb[c][e]));
+                        l += x;
+                    }
+                }
+                if constexpr (FULL) {
 #pragma unroll
-                for (int e = 0; e < 8; e += 2)
-                    l = __builtin_amdgcn_fdot2(h2{pb[c][e], pb[c][e + 1]}, ones, l, false);
+                    for (int e = 0; e < 8; e += 2)
+                        l = __builtin_amdgcn_fdot2(h2{pb[c][e], pb[c][e + 1]}, ones, l, false);
+                }
             }
 #pragma unroll
             for (int c = 0; c < BN / 16; ++c)
@@ -1218,6 +1237,8 @@ __device__ inline void tile_rows(const half_t* __restrict__ q, const half_t* __r
                     const h4 lo = lds_read_transposed(at + voff[t] / 2);
                     const h4 hi = lds_read_transposed(at + voff[NT + t] / 2);
                     const h8 va = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+                    if constexpr (!FULL)
+                        o[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(va, pl[c], o[t], 0, 0, 0);
                     o[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(va, pb[c], o[t], 0, 0, 0);
                 }
         }

@@ -4,7 +4,7 @@ hundreds of powers of two over long ranges of keys that every row sees."""
 import numpy as np
 import pytest
 
-from helpers import attention_bound
+from helpers import attention_bound, attention_exact, ulp16
 from test_gpu_paged import DTYPES, Batch, normal, packed_check
 
 pytestmark = pytest.mark.gpu
@@ -142,3 +142,56 @@ def test_light_keys_of_one_sequence(ctx, q_len, d):
                                    v[:, :, :keys - q_len + 1], 1.0 / np.sqrt(d), keys - q_len,
                                    None, "f16_fused")
     assert np.all(np.abs(got[:, :, :1] - exact) <= bound)
+
+
+def check_22_bits(q, k, v, scale, start, got):
+    """f16 outputs of probabilities that keep 22 bits (2^-22 of each, 2^-37 of the row's
+    maximum below the normal range) beside sums in f32 and the outputs' own rounding."""
+    exact, weight, _ = attention_exact(q, k, v, scale, start)
+    _, bound = attention_bound(q, k, v, scale, start, None, "f32")
+    vmax = np.max(np.abs(np.asarray(v, np.float64)))
+    bound = bound + 2.0 ** -22 * weight + k.shape[2] * 2.0 ** -37 * vmax
+    bound = bound + 0.5 * ulp16(np.abs(exact) + bound)
+    err = np.abs(np.asarray(got, np.float64) - exact)
+    worst = np.unravel_index(np.argmax(err / bound), err.shape)
+    assert np.all(err <= bound), f"error {err[worst]:.4g} > {bound[worst]:.4g} at {worst}"
+
+
+# Small query elements and few keys: the sums' roundings are then small beside those of
+# probabilities held in one f16 part.
+@pytest.mark.parametrize("n", [1, 9])
+@pytest.mark.parametrize("d", [8, 24, 40, 56, 72, 80, 88, 104, 112, 120, 32, 64, 96, 128])
+def test_probabilities_of_a_paged_batch_keep_22_bits(ctx, d, n):
+    """Of every head size where a request has few rows, of the sizes off the multiples of
+    32 where it has more."""
+    if n > 4 and d % 32 == 0:
+        n = 4  # 16 rows of four heads
+    b = Batch([(c, n) for c in (20, 3, 30, 12, 25)], 8, 2, d, 16, np.float16, ("22 bits", d, n),
+              sigma=0.25)
+    got = b.run(ctx)
+    for i, (c, _) in enumerate(b.spans):
+        rows = slice(int(b.offsets[i]), int(b.offsets[i + 1]))
+        check_22_bits(b.q[rows].transpose(1, 0, 2)[None], b.k[i].transpose(1, 0, 2)[None],
+                      b.v[i].transpose(1, 0, 2)[None], b.scale, c,
+                      got[rows].transpose(1, 0, 2)[None])
+
+
+@pytest.mark.parametrize("many", [False, True])
+@pytest.mark.parametrize("d", [8, 24, 40, 56, 72, 80, 88, 104, 112, 120])
+def test_probabilities_of_packed_prompts_keep_22_bits(ctx, d, many):
+    """Head sizes off the multiples of 32, in narrow and wide tiles."""
+    lengths = [30, 7, 25] + ([33] * 110 if many else [])
+    qh, kvh = (32, 8) if many else (8, 2)
+    tokens, heads = sum(lengths), qh + 2 * kvh
+    x = normal((tokens, heads, d), np.float32, "22 bits packed", d, many)
+    x[:, :qh] *= 0.25
+    x = x.astype(np.float16)
+    parts = x[:, :qh], x[:, qh:qh + kvh], x[:, qh + kvh:]
+    views = [(ctx.upload(np.ascontiguousarray(p)), p.shape, (p.shape[1] * d, d, 1)) for p in parts]
+    offsets = np.cumsum([0] + lengths).astype(np.uint32)
+    scale = 1.0 / np.sqrt(d)
+    got = ctx.packed_attention(*views, ctx.upload(offsets), scale, max(lengths)).numpy()
+    for i in (0, 1, 2, len(lengths) - 1):
+        rows = slice(int(offsets[i]), int(offsets[i + 1]))
+        q, k, v = (p[rows].transpose(1, 0, 2)[None] for p in parts)
+        check_22_bits(q, k, v, scale, 0, got[rows].transpose(1, 0, 2)[None])
