@@ -346,12 +346,17 @@ _context = None
 
 
 def _framework():
-    """The process's one context, as a program on one GPU holds it."""
+    """The process's one context, as a program on one GPU holds it.  Torch works on its stream
+    from then on: what writes the inputs, the calls and what reads their outputs run in the
+    order in which the program issues them."""
     global _context
     if _context is None:
         from rustllm_amd import abi
 
         _context = abi.Context(0)
+        stream = torch.cuda.ExternalStream(_context.lib.rl_context_stream(_context.handle))
+        stream.wait_stream(torch.cuda.current_stream())
+        torch.cuda.set_stream(stream)
     return _context
 
 
@@ -407,6 +412,8 @@ OWN = {"plan": _own_plan, "append": _own_append, "packed": _own_packed, "paged":
 
 
 def run(state: dict) -> dict:
+    """One pass.  With `own`, on the context's stream, which is torch's current one after the
+    first pass; a caller that turns torch to another stream orders the two."""
     case, t = state["case"], state["t"]
     if own:
         return OWN[case["op"]](_framework(), case, t, _buffers(state))
