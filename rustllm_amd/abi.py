@@ -255,13 +255,15 @@ def _u64_array(values: Sequence[int]):
 
 @functools.lru_cache(maxsize=256)
 def _u64_arrays_of(*values: tuple):
+    if any(len(v) != 3 for v in values):
+        raise ValueError(f"dims and strides of rank 3 expected, got {values}")
     arrays = [_u64_array(v) for v in values]
     return arrays, tuple(ctypes.addressof(a) for a in arrays)
 
 
 def _view_addresses(*views):
-    """The dims and strides of (buffer, dims, strides) views as C arrays: the
-    arrays (to be held over the call) and their addresses."""
+    """The dims and strides of (buffer, dims, strides) views of rank 3 as C arrays:
+    the arrays (to be held over the call) and their addresses."""
     shapes = []
     for _, dims, strides in views:
         shapes += (tuple(dims), tuple(strides))
