@@ -436,9 +436,11 @@ rl_status append_entry(rl_context* ctx, const char* name, const rl_buffer* q_src
     if (D % 2 != 0)
         return fail(RL_ERR_INVALID_SHAPE, "RoPE head size must be even, got %llu",
                     (unsigned long long)D);
-    const unsigned __int128 numel =
+    const uint64_t most = std::max({tokens, q_heads, kv_heads, D});
+    const unsigned __int128 numel =  // does not wrap if each factor is below 2^32
         (unsigned __int128)tokens * D * ((unsigned __int128)q_heads + 2 * kv_heads);
-    if (numel > UINT32_MAX) return fail(RL_ERR_INVALID_SHAPE, "append element count exceeds u32");
+    if (most > UINT32_MAX || numel > UINT32_MAX)
+        return fail(RL_ERR_INVALID_SHAPE, "append element count exceeds u32");
     if (table_rows == 0 || table_rows > UINT32_MAX)
         return fail(RL_ERR_INVALID_SHAPE, "invalid RoPE table rows %llu",
                     (unsigned long long)table_rows);

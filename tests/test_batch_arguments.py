@@ -11,8 +11,9 @@ lib = abi.load()
 SHAPE, DEVICE = 2, 9
 
 
-def buf(n, byte_len, addr=0x10000):
-    return ctypes.byref(abi.RlBuffer(addr, n, byte_len))
+def buf(n, es):
+    """An rl_buffer of n elements, lengths modulo 2^64."""
+    return abi.RlBuffer(0x10000, n % (1 << 64), n * es % (1 << 64))
 
 
 def u64s(*v):
@@ -28,3 +29,18 @@ def test_views_of_another_rank_are_refused(dims):
                   (good, (None, (4, 2, 64), dims), good), (good, good, (None, dims, dims))]:
         with pytest.raises(ValueError, match="rank 3"):
             abi._view_addresses(*views)
+
+
+@pytest.mark.parametrize("dt,es", [("f32", 4), ("f16", 2)])
+def test_append_of_counts_that_wrap(dt, es):
+    """Token and head counts of views with strides of zero whose element count is a
+    multiple of 2^128."""
+    tokens, q_heads, kv_heads, d = 1 << 63, (1 << 64) - 2, 1, 2
+    q, kv, still = u64s(tokens, q_heads, d), u64s(tokens, kv_heads, d), u64s(0, 0, 1)
+    row, table, per_token = buf(2, es), buf(8, 4), buf(tokens, 4)
+    pool = buf(3 * 4 * d, es)
+    held = [row, q, still, row, kv, still, row, kv, still, table, table, 8, per_token, per_token,
+            buf(tokens * q_heads * d, es), pool, pool]
+    status = getattr(lib, f"rl_qkv_rope_paged_append_{dt}")(
+        None, *[ctypes.addressof(x) if not isinstance(x, int) else x for x in held], 3, 4)
+    assert status == SHAPE and "exceeds u32" in abi.last_error()
