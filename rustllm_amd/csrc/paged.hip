@@ -70,7 +70,7 @@ __global__ __launch_bounds__(kPlanThreads) void k_paged_plan(
     const uint32_t* __restrict__ free_pages, uint32_t* table, uint32_t* __restrict__ offsets,
     uint32_t* __restrict__ context, uint32_t* __restrict__ slots, uint32_t* __restrict__ positions,
     uint32_t* __restrict__ taken, PlanParams p) {
-    __shared__ uint32_t first_token[kPlanThreads + 1];
+    __shared__ uint32_t first_token[kPlanThreads];
     __shared__ uint32_t first_page[kPlanThreads];
     __shared__ uint32_t had[kPlanThreads];
     __shared__ uint32_t sums[2][kPlanWaves];
@@ -114,7 +114,6 @@ __global__ __launch_bounds__(kPlanThreads) void k_paged_plan(
         first_token[t] = before;
         first_page[t] = page_before;
         had[t] = c;
-        if (t == kPlanThreads - 1) first_token[kPlanThreads] = tokens_before;
         if (live && i >= mine0 && i < mine_end) {
             offsets[i] = before;
             context[i] = add_sat(c, n);
