@@ -286,6 +286,13 @@ def _power_of_two(n: int) -> int:
     return 1 << max(n - 1, 0).bit_length()
 
 
+def _workspace_sizes(requests: int, kv_heads: int) -> tuple:
+    """What paged_attention's own workspace of a batch is made for: the next powers
+    of two, except near the library's limit (2^23 requests times KV heads)."""
+    sizes = _power_of_two(requests), _power_of_two(kv_heads)
+    return sizes if sizes[0] * sizes[1] <= 1 << 22 else (requests, kv_heads)
+
+
 class DeviceBuffer:
     """One pooled rl_buffer with the dtype/shape it was created for."""
 
@@ -687,14 +694,15 @@ class Context:
         """Attention of each request's rows of q [tokens, QH, D] over its pages
         of the [pages, KVH, page_size, D] pools.  Without a `workspace` the
         context makes and keeps its own, one for each power of two of requests
-        and KV heads (so a step to be recorded runs once before); a graph that is
-        replayed on another context needs one of its own."""
+        and KV heads (for each size above 2^22 of their product), so a step to be
+        recorded runs once before; a graph that is replayed on another context
+        needs one of its own."""
         tokens, qh, hd = q.shape
         pages, kvh, page_size, _ = k_pages.shape
         requests, blocks = table.shape
         out = out or self.empty(q.shape, q.dtype)
         if workspace is None:
-            sizes = (_power_of_two(requests), _power_of_two(kvh))
+            sizes = _workspace_sizes(requests, kvh)
             workspace = self._workspaces.get(sizes)
             if workspace is None:
                 workspace = self._workspaces[sizes] = self.paged_workspace(*sizes)

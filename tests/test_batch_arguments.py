@@ -44,3 +44,15 @@ def test_append_of_counts_that_wrap(dt, es):
     status = getattr(lib, f"rl_qkv_rope_paged_append_{dt}")(
         None, *[ctypes.addressof(x) if not isinstance(x, int) else x for x in held], 3, 4)
     assert status == SHAPE and "exceeds u32" in abi.last_error()
+
+
+@pytest.mark.parametrize("requests,kv_heads", [
+    (1, 1), (3, 3), (64, 8), (2_100_000, 3), (5_000_000, 1), (1, 8_000_000), (699_050, 11)])
+def test_the_bindings_workspace_fits_every_batch_a_call_takes(requests, kv_heads):
+    """Sizes that rl_paged_attention_* accepts, rounded up or not, are accepted for the
+    workspace that the binding makes."""
+    made = abi._workspace_sizes(requests, kv_heads)
+    assert made[0] >= requests and made[1] >= kv_heads
+    for sizes in ((requests, kv_heads), made):
+        status = lib.rl_paged_attention_workspace(None, *sizes, ctypes.byref(abi.RlBuffer()))
+        assert status == DEVICE, (sizes, abi.last_error())
