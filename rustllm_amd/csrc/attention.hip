@@ -48,7 +48,6 @@
 namespace rl {
 namespace {
 
-constexpr float kLog2e = 1.44269504088896340736f;
 constexpr float kLn2 = 0.693147180559945309417f;
 
 struct AttnParams {
@@ -72,14 +71,6 @@ struct AttnParams {
 };
 
 // ------------------------------------------------------------- MFMA kernel
-
-// max over lanes l and l ^ 32 without an LDS permute: v_permlane32_swap
-// returns {lower lane's value, upper lane's value} in both lanes.
-__device__ inline float max_halves(float v) {
-    const auto s = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v),
-                                                    false, false);
-    return fmaxf(__uint_as_float(s[0]), __uint_as_float(s[1]));
-}
 
 // Buffer resource (gfx9 descriptor: base, stride 0, size in bytes, 32-bit
 // data format) for raw loads from `base`: a load at or past `bytes` returns
@@ -1545,24 +1536,6 @@ __global__ __launch_bounds__(64 * kSplitWaves) void k_attention_split(
 // k_attention_split.
 __device__ inline uint32_t key16(uint32_t m, uint32_t a) {
     return 32 * (m / 2) + 8 * (a / 4) + 4 * (m % 2) + a % 4;
-}
-
-// max / sum over lanes l, l ^ 16, l ^ 32, l ^ 48 (one query row's four
-// lane groups).  A swap returns {lower lane's value, upper lane's value} in
-// both lanes of a pair, so both compute the same result bit for bit.
-__device__ inline float rows4_max(float v) {
-    auto s = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false,
-                                              false);
-    v = fmaxf(__uint_as_float(s[0]), __uint_as_float(s[1]));
-    s = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-    return fmaxf(__uint_as_float(s[0]), __uint_as_float(s[1]));
-}
-__device__ inline float rows4_sum(float v) {
-    auto s = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false,
-                                              false);
-    v = __uint_as_float(s[0]) + __uint_as_float(s[1]);
-    s = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-    return __uint_as_float(s[0]) + __uint_as_float(s[1]);
 }
 
 // Chunk swizzle of the decode's value stage (rows of D halves, 16-byte

@@ -1,5 +1,5 @@
-// mfma_layout.hpp -- operand layouts shared by the matrix-core kernels of
-// attention.hip and gqa.hip (gfx950, wave64).
+// mfma_layout.hpp -- operand layouts and lane reductions shared by the matrix-core
+// kernels of attention.hip, ragged_attention.hip and gqa.hip (gfx950, wave64).
 //
 // v_mfma_f32_32x32x16_f16 and _bf16 take A / B operands
 // with lane l holding row (A) or column (B) l % 32 and the inner-dimension
@@ -14,6 +14,8 @@
 
 namespace rl {
 namespace {
+
+constexpr float kLog2e = 1.44269504088896340736f;
 
 typedef half_t h8 __attribute__((ext_vector_type(8)));
 typedef half_t h4 __attribute__((ext_vector_type(4)));
@@ -69,6 +71,32 @@ __device__ inline h4 lds_read_transposed(const half_t* p) {
 // are not: the compiler counts them for its own instructions only.
 __device__ inline float max3(float a, float b, float c) {
     return __builtin_elementwise_maximumnum(__builtin_elementwise_maximumnum(a, b), c);
+}
+
+// max over lanes l and l ^ 32 without an LDS permute: v_permlane32_swap
+// returns {lower lane's value, upper lane's value} in both lanes.
+__device__ inline float max_halves(float v) {
+    const auto s = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v),
+                                                    false, false);
+    return fmaxf(__uint_as_float(s[0]), __uint_as_float(s[1]));
+}
+
+// max / sum over lanes l, l ^ 16, l ^ 32, l ^ 48 (one query row's four
+// lane groups).  A swap returns {lower lane's value, upper lane's value} in
+// both lanes of a pair, so both compute the same result bit for bit.
+__device__ inline float rows4_max(float v) {
+    auto s = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false,
+                                              false);
+    v = fmaxf(__uint_as_float(s[0]), __uint_as_float(s[1]));
+    s = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return fmaxf(__uint_as_float(s[0]), __uint_as_float(s[1]));
+}
+__device__ inline float rows4_sum(float v) {
+    auto s = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false,
+                                              false);
+    v = __uint_as_float(s[0]) + __uint_as_float(s[1]);
+    s = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return __uint_as_float(s[0]) + __uint_as_float(s[1]);
 }
 
 // f32 products on the bf16 matrix cores (v_mfma_f32_32x32x16_bf16, 16 times

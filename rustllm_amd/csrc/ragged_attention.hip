@@ -26,8 +26,6 @@
 namespace rl {
 namespace {
 
-constexpr float kLog2e = 1.44269504088896340736f;
-
 // Added to the exponent of a probability that is rounded to f16, in the sum as in
 // the product, so that it cancels in their quotient: f16's normal range then reaches
 // down to 2^-26 of the row's maximum, and what is rounded away below it is at most
@@ -341,19 +339,6 @@ constexpr int kSplitWaves = 4;
 constexpr uint32_t kTicketStride = 64;
 constexpr uint64_t kStreamKeyBytes = uint64_t(100) << 20;
 
-__device__ inline float columns_max(float v) {  // over lanes l, l ^ 16, l ^ 32, l ^ 48
-    auto s = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-    v = fmaxf(__uint_as_float(s[0]), __uint_as_float(s[1]));
-    s = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-    return fmaxf(__uint_as_float(s[0]), __uint_as_float(s[1]));
-}
-__device__ inline float columns_sum(float v) {
-    auto s = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-    v = __uint_as_float(s[0]) + __uint_as_float(s[1]);
-    s = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-    return __uint_as_float(s[0]) + __uint_as_float(s[1]);
-}
-
 // Agent-coherent pairs of floats: written through, and read past, an XCD's L2.
 __device__ inline void publish2(float* p, float a, float b) {
     const uint64_t w = uint64_t(__float_as_uint(a)) | uint64_t(__float_as_uint(b)) << 32;
@@ -614,7 +599,7 @@ __device__ inline void split_rows(const T* __restrict__ q, const T* __restrict__
                 s[t][e] = at <= seen ? s[t][e] : -INFINITY;
                 mx = fmaxf(mx, s[t][e]);
             }
-        mx = columns_max(mx) * p.scale_log2;
+        mx = rows4_max(mx) * p.scale_log2;
         const float m_new = fmaxf(m, mx);
         const float shift = m_new == -INFINITY ? 0.0f : m_new;
         const float alpha = __builtin_amdgcn_exp2f(m - shift);
@@ -690,7 +675,7 @@ __device__ inline void split_rows(const T* __restrict__ q, const T* __restrict__
         walk(std::true_type{});
     else
         walk(std::false_type{});
-    l = columns_sum(l);
+    l = rows4_sum(l);
     if (__any(bad_page)) l = NAN;  // row_by_wave finds which rows see it
 
     // the four waves' states -> the range's.  Lane (g, lr), f16: elements
@@ -871,12 +856,6 @@ __device__ inline void load_to_lds(const void* from, uint32_t lds) {
         : "memory");
 }
 
-// max over lanes l and l ^ 32
-__device__ inline float halves_max(float v) {
-    const auto s = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false,
-                                                    false);
-    return fmaxf(__uint_as_float(s[0]), __uint_as_float(s[1]));
-}
 // Zeros for the chunks of a padded K row.
 __device__ __align__(16) const uint32_t zero_chunk[4] = {0, 0, 0, 0};
 
@@ -1196,7 +1175,7 @@ __device__ inline void tile_rows(const half_t* __restrict__ q, const half_t* __r
                     mx = max3(mx, s[kt][e], s[kt][e + 1]);
                     my = max3(my, s[kt][e + 2], s[kt][e + 3]);
                 }
-            mx = halves_max(fmaxf(mx, my)) * p.scale_log2;
+            mx = max_halves(fmaxf(mx, my)) * p.scale_log2;
             if (__any(mx > m + kSlack)) {
                 const float m_new = fmaxf(m, mx);
                 const float alpha = m_new > m ? __builtin_amdgcn_exp2f(m - m_new) : 1.0f;
@@ -1509,7 +1488,7 @@ __device__ inline void tile_rows_f32(const float* __restrict__ q, const float* _
             mx = max3(mx, s[i], s[i + 1]);
             my = max3(my, s[i + 2], s[i + 3]);
         }
-        mx = halves_max(fmaxf(mx, my)) * scale_log2;
+        mx = max_halves(fmaxf(mx, my)) * scale_log2;
         if (__any(mx > m + kSlack)) {
             const float m_new = fmaxf(m, mx);
             const float alpha = m_new > m ? __builtin_amdgcn_exp2f(m - m_new) : 1.0f;
