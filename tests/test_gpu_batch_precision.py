@@ -195,3 +195,42 @@ def test_probabilities_of_packed_prompts_keep_22_bits(ctx, d, many):
         rows = slice(int(offsets[i]), int(offsets[i + 1]))
         q, k, v = (p[rows].transpose(1, 0, 2)[None] for p in parts)
         check_22_bits(q, k, v, scale, 0, got[rows].transpose(1, 0, 2)[None])
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("n,cached", [(1, 5000), (2, 300), (40, 900), (300, 500)])
+@pytest.mark.parametrize("d", [64, 128, 80])
+def test_scores_of_tens_of_millions_take_one_key(ctx, dtype, n, cached, d):
+    """Scores so large that f32's steps between them are whole exponents: each row's
+    output is the value row v of its largest score wherever the next one is far below it.
+    The weight p of that key is not 1 but 2 to what the maximum's rounding left, in the sum
+    as in the product: (p v) / p.  In f32 that is v up to the roundings of p v, of the
+    quotient's two steps, of both sides' rescaling in two merges, and the split's: 8 of
+    2^-24.  In f16 the rounding of the output takes it back to v."""
+    b = Batch([(cached, n), (30, 1)], 4, 2, d, 32, dtype, ("millions", n, d), sigma=1e4)
+    for i in range(2):
+        b.k[i] = (1e3 * b.k[i].astype(np.float32)).astype(dtype)
+        pos = np.arange(b.context[i])
+        b.kp[b.table[i, pos // 32], :, pos % 32] = b.k[i]
+    assert np.isfinite(b.q).all() and np.isfinite(b.k[0]).all()
+    got = b.run(ctx)
+    checked = 0
+    for i, (c, m) in enumerate(b.spans):
+        for j in range(m):
+            row = int(b.offsets[i]) + j
+            for h in range(4):
+                s = b.k[i][:c + j + 1, h // 2].astype(np.float64) @ b.q[row, h].astype(np.float64)
+                s *= b.scale
+                top = int(np.argmax(s))
+                s[top], best = -np.inf, s[top]
+                # errors of two scores of D products each: D 2^-24 of their terms' sum
+                terms = np.abs(b.q[row, h].astype(np.float64)) @ np.abs(
+                    b.k[i][:c + j + 1, h // 2].astype(np.float64)).T
+                unsure = 2 * b.scale * d * 2.0 ** -24 * terms.max()
+                if best - np.max(s, initial=-np.inf) < unsure + 200:
+                    continue
+                v = b.v[i][top, h // 2].astype(np.float64)
+                off = 8 * 2.0 ** -24 * np.abs(v) if dtype == np.float32 else 0.0
+                assert np.all(np.abs(got[row, h] - v) <= off), (i, j, h)
+                checked += 1
+    assert checked > 2 * n
