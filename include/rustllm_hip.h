@@ -552,7 +552,19 @@ rl_status rl_gqa_pv_matmul_f16(rl_context* ctx, const rl_buffer* probs, const rl
  * offsets[i + 1] of every [tokens, heads, head_dim] tensor.  An attention call
  * is one launch and refused past its size: 8 tokens q_heads + 512 sequences
  * kv_heads + 2^17 up to 2^32 - 1, and tokens q_heads below 2^26 where head size,
- * strides, alignment or pages of fewer than 8 rows rule the matrix cores out. */
+ * strides, alignment or pages of fewer than 8 rows rule the matrix cores out.
+ *
+ * What the speed rests on.  The matrix cores serve head sizes of whole 16-byte
+ * pieces up to 128 elements, pages of at least 8 rows (and less than 4 GiB) and,
+ * packed, strides and starts on the 16-byte grid; everything else runs on vector
+ * instructions, a wave for each row and head, a hundred times slower (16 single
+ * tokens of up to 4000 keys, 32/8 heads: 34 us at head size 128, 7.0 ms at 256,
+ * 3.6 ms with pages of 4; 4 prompts of up to 1024: 24 us, 2.2 ms off the grid).
+ * The keys of a request of up to 16 rows a KV head (rows times q_heads / kv_heads)
+ * are shared out over the GPU.  With more rows a workgroup walks all the keys of
+ * its tile of 32 to 256 rows, so that few rows over a long context take long
+ * (100 thousand keys, 32/8 heads of 128: 4 new tokens 96 us, 5 or 512 of them 1.5 to
+ * 1.6 ms; one token of 32 heads on one KV head 1.4 ms). */
 #define RL_NO_PAGE 0xffffffffu
 #define RL_NO_SLOT 0xffffffffu
 
@@ -613,13 +625,15 @@ rl_status rl_paged_attention_workspace(rl_context* ctx, uint64_t sequences, uint
  * context[i] - n + j (n its rows) and sees the keys at positions up to its
  * own.  q, out: contiguous [tokens, q_heads, head_dim].  No request has more
  * than max_queries rows or max_context positions (at most max_blocks *
- * page_size).  Rows of no request (and past a request's first max_queries)
- * are not written; a row that sees no key (a position below 0) is zeros; a
- * row that sees a key of a page at or past `pages`, and every row of a
- * request whose context passes max_context, is NaN.  Types, roundings and
- * head sizes as rl_attention_*; the f16 probabilities of requests of up to 16
- * rows a KV head (rows times q_heads / kv_heads) have 22 bits for every head
- * size.  May be recorded into a graph, the workspace made before. */
+ * page_size); the bounds may be loose, though max_queries beyond 16 rows a KV
+ * head costs a batch of single tokens up to an eighth more time.  Rows of no
+ * request (and past a request's first max_queries) are not written; a row that
+ * sees no key (a position below 0) is zeros; a row that sees a key of a page at
+ * or past `pages`, and every row of a request whose context passes max_context,
+ * is NaN.  Types, roundings and head sizes as rl_attention_*; the f16
+ * probabilities of requests of up to 16 rows a KV head have 22 bits for every
+ * head size, and those of either batch attention are kept to 2^-37 of the row's
+ * largest.  May be recorded into a graph, the workspace made before. */
 rl_status rl_paged_attention_f32(rl_context* ctx, const rl_buffer* q, const rl_buffer* k_pages,
                                  const rl_buffer* v_pages, const rl_buffer* block_table,
                                  const rl_buffer* offsets, const rl_buffer* context,

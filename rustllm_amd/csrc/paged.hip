@@ -33,7 +33,7 @@ namespace {
 // table entry.  Every other read of the table is of an entry that the plan
 // does not write.  Bound by latency: two dependent reads (lengths, then
 // table or free list) and the scan's two barriers: 3.3 us for 48 requests of one
-// token, 4.4 for 480 with 49 thousand tokens (a call 4.7; 8.5 with a workgroup for
+// token, 4.5 for 480 with 49 thousand tokens (a call 5.3; 8.5 with a workgroup for
 // 8192 tokens instead of 1024).
 constexpr int kPlanThreads = 1024;
 constexpr int kPlanWaves = kPlanThreads / 64;
@@ -398,7 +398,11 @@ void launch_append(rl_context* ctx, uint64_t tokens, uint64_t heads, AppendParam
     // One MI355X, 32/8 heads of 128 in f16, a thread a head / four / two and streamed
     // loads: 543 tokens 5.8 / 5.9 us; 1055, 6.9 / 5.9; 2079 (26 MB of rows) 10.7 / 9.6
     // / 10.7, 10.3 with four and plain stores; 5663 (70 MB) - / 21.9 / 25.2; 8223 (101
-    // MB) - / 37.2 / 35.2, 44.3 with four and plain stores.
+    // MB) - / 37.2 / 35.2, 44.3 with four and plain stores.  Other heads: 15/5 of 64 in f16,
+    // 4127 tokens 7.3 / 6.0 / 7.2, 24607 (79 MB) 34.1 / 29.4 / 33.2, 34847 (112 MB) 45.5 /
+    // 43.4 / 45.3; 32/8 of 128 in f32, 543 tokens 6.7 / 5.9 / 6.1, 2079 (51 MB) 21.4 / 16.5 /
+    // 18.5, 4127 (101 MB) 41.2 / 35.6 / 34.4, 6175 (152 MB) 58.5 / 54.4 / 50.4; 9/3 of 64
+    // in f32, 8223 (32 MB) 12.7 / 11.1 / 12.2, 30751 (118 MB) 47.5 / 44.2 / 41.0.
     const bool many = tokens * heads * packs >= uint64_t(ctx->num_cus) * 1024;
     const bool stream = many && tokens * heads * 2 * p.half_dim * sizeof(T) >= kStreamRows;
     const uint64_t steps = ceil_div(heads, stream ? 2 : many ? 4 : 1);

@@ -305,8 +305,8 @@ __global__ __launch_bounds__(64) void k_ragged_rows(const T* __restrict__ q,
 // and products (V) are through, so the next block's rows are in flight under
 // the rest of the work; its page entries are read a block ahead.  Bound by HBM:
 // 155 us for 934 MB (60 requests of up to 8000 keys, 32/8 heads of 128 in f16; 6.0
-// TB/s, where a plain read runs at 6.2 to 6.4), 74.6 us for one request of 100,003
-// keys (5.5 TB/s); one request of 1536 keys takes 7.2 us, most of it the launch, three
+// TB/s, where a plain read runs at 6.2 to 6.4), 75 us for one request of 100,003
+// keys (5.5 TB/s); one request of 1536 keys takes 7.3 us, most of it the launch, three
 // dependent reads and the hand-over.  Equal shares against each request cut by
 // itself: 44 -> 40 us for 64 requests of up to 4000 keys (15/5 heads of 64).
 // Registers refilled in place leave two waves a SIMD; three spill (174 -> 243 us).
@@ -829,10 +829,11 @@ __device__ inline void split_rows(const T* __restrict__ q, const T* __restrict__
 // different KV heads, so that one XCD's workgroups (every eighth) share rows of
 // K and V in its L2.
 //
-// Bound by vector work (the softmax) beside the products, with two waves a SIMD:
-// 350 us for 8 prompts of up to 4096 tokens (32/8 heads of 128, 302 GFLOP: 860
-// TFLOP/s, where a large f16 matrix product runs at 1196), the matrix cores busy 41 %
-// of the cycles, the vector ALUs 47 %, LDS 21 % without bank conflicts.  Slower:
+// Bound by how little the products and the softmax overlap: every block's barrier
+// brings all waves of a workgroup to the same phase, with two or three waves a SIMD.
+// Takes 354 to 366 us for 8 prompts of up to 4096 tokens (32/8 heads of 128, 302 GFLOP: 825
+// to 850 TFLOP/s, where a large f16 matrix product runs at 1196), the matrix cores busy
+// 41 % of the cycles, the vector ALUs 47 %, LDS 21 % without bank conflicts.  Slower:
 // the next block's scores beside this one's softmax (356 -> 372 to 391 us), wave
 // priorities around the products (no change), 128-key blocks for head size 64 (564 -> 621 us
 // for 60 prompts).
@@ -1644,8 +1645,8 @@ __global__ __launch_bounds__(64 * QW * KS, (Tile<T, NT, QW, KS, BN>::kWaves)) vo
 // A paged batch of chunks and single tokens in one launch: the first
 // split_blocks workgroups stream the keys of the requests of few rows, the
 // others take tiles, so that the one's wait for memory runs beside the other's
-// products (one MI355X: 65.5 us as two launches, 57 as one, 45.5 with the longest tiles
-// first, for 4 chunks of 509 tokens and 20 single tokens over up to 4000 keys).
+// products (one MI355X: 65.5 us as two launches, 57 as one, 45.5 to 46.8 with the longest
+// tiles first, for 4 chunks of 509 tokens and 20 single tokens over up to 4000 keys).
 template <typename T, int NT, int QW, int KS, int BN, bool FULL>
 __global__ __launch_bounds__(64 * QW * KS, (Tile<T, NT, QW, KS, BN>::kWaves)) void k_paged_mixed(
     const T* __restrict__ q, const T* __restrict__ k, const T* __restrict__ v,
@@ -1771,7 +1772,10 @@ void launch_tiles(rl_context* ctx, const T* q, const T* k, const T* v, T* out,
 //   f16, paged, whose other part takes places too: QW 4 from half of `slots` on, 2 x 2
 //     below: 55.4 / 49.2 [350], 65.2 / 76 [700]; D 128 67.5 / 71.4 [296].  Below half
 //     a tile a CU, 1 x 4 at 64: 24.6 / 28.6 [35], 32.5 / 31.8 [80], 27.2 / 30.2
-//     [115]; 40.1 / 32.6 [175].
+//     [115]; 40.1 / 32.6 [175].  Not at 128, where its LDS leaves one workgroup a CU:
+//     36.5 / 45.0 [5], 44.1 / 47.4 [50], but 73.2 / 49.2 [75], and 18.9 / 16.2 [40] over
+//     up to 500 keys.  At 96 and 32, where 2 x 2 is used, it would be the faster one:
+//     39.5 / 43.6 [5], 42.2 / 45.9 [19] and 17.0 / 20.1 [5], 19.8 / 24.1 [56].
 //   f32: 1 x 4 below a tile a CU, 2 x 2 from there on (4 x 1 for more than 64 elements):
 //     24.5 / 30.7 [155], 61.7 / 49.7 [445]; D 128 50.7 / 53.9 [144], 116 / 76.4 [352].
 // Longest tiles first (a search over the lengths in every workgroup, about 0.7 us)
@@ -1995,7 +1999,10 @@ rl_status paged_entry(rl_context* ctx, const char* name, const rl_buffer* q,
         }
         // beside tiles: half of the workgroups that would fill the CUs (60 single tokens of
         // up to 8000 keys and a chunk of 30 tokens: 183 us, a quarter 295; 4 chunks and
-        // 20 single tokens of up to 4000 keys: 57 / 56)
+        // 20 single tokens of up to 4000 keys: 57 / 56).  The host knows the bound alone, so
+        // a batch of single tokens under a loose one has as few: 36.9 -> 41.8 us for 64 of
+        // up to 4000 keys (15/5 heads of 64), 16.4 -> 18.2 for 16 of up to 1500 (32/8 of
+        // 128), 155.8 -> 156.8 for 60 of up to 8000.
         p.slots = uint32_t(std::max<uint64_t>(slots / 2, 1));
         split_blocks = p.slots * p.kv_heads;
     }
