@@ -579,6 +579,8 @@ rl_status rl_gqa_pv_matmul_f16(rl_context* ctx, const rl_buffer* probs, const rl
  *     RL_NO_SLOT for a token whose page is missing, at or past `pages` or past
  *     the table row, and for rows behind the last request's
  *   taken[0]: pages needed; more than free_pages holds = some tokens have none
+ *     (entries at or past `pages`, such as RL_NO_PAGE, hold none: a recorded plan,
+ *     whose list keeps its length, has the list filled up with them)
  * `tokens` (the length of slots and positions) is at least the sum of fresh;
  * tokens past it, and pages that start past it, are not planned.  Sums stop at
  * 2^32 - 1. */

@@ -4,7 +4,7 @@ import numpy as np
 import pytest
 
 from helpers import attention_bound
-from test_gpu_paged import DTYPES, NONE, normal
+from test_gpu_paged import DTYPES, NONE, Batch, normal, packed_check
 
 pytestmark = pytest.mark.gpu
 
@@ -38,3 +38,46 @@ def test_paged_attention_of_millions_of_requests(ctx, dtype, n):
         err = np.abs(got[at * n:(at + 1) * n].astype(np.float64).transpose(1, 0, 2) - exact[0])
         assert np.all(err <= bound[0]), i
     ctx._workspaces.pop((requests, kvh)).release()  # 1.5 GiB of counters
+
+
+@pytest.mark.parametrize("dtype,d", [(np.float32, d) for d in range(4, 129, 4)]
+                         + [(np.float16, d) for d in range(8, 129, 8)])
+def test_every_head_size_of_the_matrix_kernels(ctx, dtype, d):
+    """Single tokens, a chunk, both in one call and packed prompts, at every head size of
+    whole 16-byte pieces."""
+    for n in (1, 25):
+        b = Batch([(70, n), (300, 1), (0, 1)], 6, 2, d, 8, dtype, ("sizes", d, n), padding=1)
+        b.check(b.run(ctx))
+    packed_check(ctx, [40, 1, 90], 6, 2, d, dtype, ("sizes", d), padding=2)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("page", [1 << 10, 1 << 14])
+@pytest.mark.parametrize("n", [1, 30])
+def test_pages_longer_than_a_context(ctx, dtype, page, n):
+    b = Batch([(700, n), (0, n), (1100, n)], 6, 2, 64, page, dtype, ("pages", page, n))
+    b.check(b.run(ctx))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("d", [64, 24, 7])
+def test_packed_keys_that_heads_share_by_a_stride_of_zero(ctx, dtype, d):
+    """K and V views whose heads are one row each (stride 0), Q's heads outside its
+    tokens."""
+    lengths, qh, kvh = [33, 1, 80], 6, 2
+    tokens = sum(lengths)
+    q = normal((qh, tokens, d), dtype, "shared", "q", d)  # heads outside tokens
+    k, v = (normal((tokens, d), dtype, "shared", s, d) for s in "kv")
+    offsets = np.cumsum([0] + lengths).astype(np.uint32)
+    scale = 1.0 / np.sqrt(d)
+    got = ctx.packed_attention((ctx.upload(q), (tokens, qh, d), (d, tokens * d, 1)),
+                               (ctx.upload(k), (tokens, kvh, d), (d, 0, 1)),
+                               (ctx.upload(v), (tokens, kvh, d), (d, 0, 1)),
+                               ctx.upload(offsets), scale, max(lengths)).numpy()
+    for i, n in enumerate(lengths):
+        rows = slice(int(offsets[i]), int(offsets[i + 1]))
+        exact, bound = attention_bound(q[None, :, rows], k[None, None, rows], v[None, None, rows],
+                                       scale, 0, None,
+                                       "f16_fused" if dtype == np.float16 else "f32")
+        err = np.abs(got[rows].astype(np.float64).transpose(1, 0, 2) - exact[0])
+        assert np.all(err <= bound[0]), i
